@@ -574,6 +574,55 @@ const char *moe355_layer_kernel_name(const moe355_layer *layer /* host */, int64
 /* 1: that launch gates and quantises the tokens as well; 0: a launch in front of it does. */
 int moe355_layer_gates_inside(const moe355_layer *layer /* host */, int64_t num_tokens);
 
+/* ---------------------------------------------------------------------------
+ * MXFP4: 32 values along a row share a power of two (one byte, exponent + 127: E8M0) and have four bits each (E2M1), the
+ * first value of a byte in its low half.  Quantisation of a block whose largest magnitude is a: exponent
+ * max(floor(log2 a) - 2, -127) (a = 0: -127), codes rounded to nearest even, magnitudes above 6 to 6; a block with an
+ * infinity or NaN: scale byte 255, which stands for NaN, codes 0.
+ * Stand in for torch_npu.npu_dynamic_mx_quant and its inverse (the MXFP4 branch of vllm_ascend/device/device_op.py:192-206).
+ * cols % 32 == 0 and at most 2^20; x, out 16-byte and codes 4-byte aligned (MOE355_E_SHAPE otherwise).
+ * x [rows, cols] fp32 / bf16 / fp16 -> codes [rows, cols / 2], scale [rows, cols / 32]; and back. */
+int moe355_dynamic_mx_quant(const void *x, int x_dtype, int64_t rows, int64_t cols, uint8_t *codes, uint8_t *scale,
+                            void *stream);
+int moe355_mx_dequant(const uint8_t *codes, const uint8_t *scale, int64_t rows, int64_t cols, void *out, int out_dtype,
+                      void *stream);
+
+/* Residual addition, RMS norm and quantisation in one pass over the rows:
+ *   x = half(x1 + x2) (x2 NULL: x1), y = half(f32(x / sqrt(mean(x^2) + epsilon) * gamma (+ beta))), computed in 64 bits,
+ *   q, scale = what moe355_dynamic_quant (MOE355_NORM_INT8: int8, fp32 [rows]) or moe355_dynamic_mx_quant
+ *   (MOE355_NORM_MXFP4) make of y; MOE355_NORM_PLAIN: y alone.
+ * x1, x2, x, y [rows, cols] of x_dtype (bf16 / fp16); gamma, beta [cols] of weight_dtype (x_dtype or fp32), beta may be
+ * NULL.  x and y may be NULL (not wanted; MOE355_NORM_PLAIN needs y); x may be the same buffer as x1 or x2.
+ * cols % 8 == 0 (MXFP4: 32) and at most 2^20; rows 16-byte aligned. */
+enum { MOE355_NORM_PLAIN = 0, MOE355_NORM_INT8 = 1, MOE355_NORM_MXFP4 = 2 };
+int moe355_add_rms_norm_quant(const void *x1, const void *x2, const void *gamma, const void *beta, int x_dtype,
+                              int weight_dtype, int64_t rows, int64_t cols, double epsilon, int kind, void *x, void *y,
+                              void *q, void *scale, void *stream);
+
+/* Weights [E, n, k / 2] codes and [E, n, k / 32] scales to the storage of the products below: as many bytes of codes, and
+ * E * n * ceil(k / 256) * 8 bytes of scales.  n % 32 == 0, k % 64 == 0. */
+int moe355_format_cast_mx(const uint8_t *codes, const uint8_t *scale, int64_t num_experts, int64_t n, int64_t k,
+                          uint8_t *codes_out, uint8_t *scale_out, void *stream);
+
+/* Grouped products of MXFP4 rows with MXFP4 weights (moe355_format_cast_mx), accumulated in fp32.
+ *   moe355_gmm_mx:               out [rows, n] = half(x . w)
+ *   moe355_gmm_mx_swiglu_quant:  y = silu(gate) * up with gate = x . w[: n / 2], up = x . w[n / 2 :] (swiglu_limit > 0 clamps
+ *                                gate to <= L and up to [-L, L]), rounded once to fp32; out [rows, n / 4] codes and
+ *                                out_scale [rows, n / 64] of its MXFP4 form
+ * Stand in for torch_npu.npu_grouped_matmul and npu_grouped_matmul_swiglu_quant_v2 with E8M0 scales (the MXFP4 branch of
+ * vllm_ascend/device/device_op.py:208-291).
+ * Row r of the sorted rows is row row_token[r] of x (NULL: row r, x_rows = rows); one outside [0, x_rows) counts as zeros.
+ * The group list (int64, meaning as above; NULL: one expert, all rows) is cut to [0, rows); rows behind the last group are left as they were.
+ * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; x, w, out 16-byte aligned. */
+size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int64_t k, int num_experts);
+int moe355_gmm_mx(const uint8_t *x, const uint8_t *x_scale, const int32_t *row_token, int64_t x_rows, const uint8_t *w,
+                  const uint8_t *w_scale, const int64_t *group_list, int group_list_type, int64_t rows, int64_t k, int64_t n,
+                  int num_experts, void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+int moe355_gmm_mx_swiglu_quant(const uint8_t *x, const uint8_t *x_scale, const int32_t *row_token, int64_t x_rows,
+                               const uint8_t *w, const uint8_t *w_scale, const int64_t *group_list, int group_list_type,
+                               int64_t rows, int64_t k, int64_t n, int num_experts, float swiglu_limit, uint8_t *out,
+                               uint8_t *out_scale, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

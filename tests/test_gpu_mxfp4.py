@@ -1,0 +1,535 @@
+"""The MXFP4 operators and the norm on the GPU against their definition in 64 bits.  What is compared is equal bit for bit: sums
+of products of four-bit values are exact in 32 bits for scales a few powers of two apart (24 bits hold K * 36 / 0.25 * 2^spread
+for every K and spread here that matters: a sum's typical size is sqrt(K) * 8 units, 2^10 for K = 7168, times 2^(2 * spread)), and
+what is rounded is rounded once from the value of the formula."""
+import numpy as np
+import pytest
+import torch
+
+import _mxfp4 as ref
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+HALF = [torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def K():
+    from vllm_ascend_amd import kernels
+
+    return kernels
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from vllm_ascend_amd import npu_ops
+
+    return npu_ops
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+    return t if dtype is None else t.to(dtype)
+
+
+def same_bits(a, b):
+    return torch.equal(a.cpu().view(torch.int16), b.cpu().view(torch.int16))
+
+
+# ------------------------------------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("shape", [(1, 32), (3, 96), (37, 1408), (2, 5, 7168), (513, 64), (1, 8224)], ids=str)
+def test_mx_quant(ops, dtype, shape):
+    say("mx_quant", dtype, shape)
+    g = torch.Generator().manual_seed(sum(shape))
+    x = torch.randn(shape, generator=g) * torch.exp2(torch.randint(-9, 9, (*shape[:-1], 1), generator=g).float())
+    x = x.to(dtype)
+    codes, scale = ops.npu_dynamic_mx_quant(x.to(DEV))
+    c, s = ref.quantise(x.double().numpy())
+    assert codes.shape == (*shape[:-1], shape[-1] // 2) and scale.shape == (*shape[:-1], shape[-1] // 32)
+    assert np.array_equal(codes.cpu().numpy(), ref.pack(c)) and np.array_equal(scale.cpu().numpy(), s)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_mx_quant_borders_and_special_values(ops, dtype):
+    say("mx_quant borders", dtype)
+    info = torch.finfo(dtype)
+    rows = []
+    borders = [0.25, 0.5, 0.75, 1.0, 1.25, 1.5, 1.75, 2.0, 2.5, 3.0, 3.5, 4.0, 5.0, 6.0, 7.0]
+    for power in (0, -3, 5):
+        for b in borders:  # the border, its neighbours of the type, under a largest value that fixes the scale
+            t = torch.tensor([b], dtype=torch.float64).to(dtype)
+            up, down = t * (1 + info.eps), t * (1 - info.eps / 2)
+            block = torch.cat([t, up, down, -t, -up, -down, torch.tensor([4.0, 0.0, -0.0], dtype=dtype)])
+            rows.append(torch.cat([block.double() * 2.0 ** power, torch.zeros(32 - len(block)).double()]))
+    rows.append(torch.zeros(32).double())
+    rows.append(-torch.zeros(32).double())
+    for v in (info.max, info.tiny, info.smallest_normal, float(torch.finfo(dtype).smallest_normal) / 4):
+        rows.append(torch.linspace(-1, 1, 32).double() * v)
+    for v in (float("inf"), -float("inf"), float("nan")):
+        r = torch.linspace(-1, 1, 32).double()
+        r[7] = v
+        rows.append(r)
+    x = torch.stack(rows).to(dtype)
+    codes, scale = ops.npu_dynamic_mx_quant(x.to(DEV))
+    c, s = ref.quantise(x.double().numpy())
+    assert np.array_equal(scale.cpu().numpy(), s)
+    assert np.array_equal(codes.cpu().numpy(), ref.pack(c))
+
+
+def test_mx_quant_of_views(ops):
+    """Transposed rows, and rows that start at an address no wide load may start at."""
+    say("mx_quant views")
+    x = torch.randn(64, 96, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    flat = torch.empty(32 * 5 + 1, dtype=torch.bfloat16, device=DEV)
+    flat.copy_(torch.arange(161) / 7)
+    for v in (x.t(), x[:, :64], x[::2], flat[1:].view(5, 32)):
+        c, s = ref.quantise(v.double().cpu().numpy())
+        codes, scale = ops.npu_dynamic_mx_quant(v)
+        assert np.array_equal(codes.cpu().numpy(), ref.pack(c)) and np.array_equal(scale.cpu().numpy(), s)
+    codes, scale = ops.npu_dynamic_mx_quant(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV))
+    assert codes.shape == (0, 32) and scale.shape == (0, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_mx_dequant_of_every_code_and_scale(ops, dtype):
+    say("mx_dequant", dtype)
+    code = np.tile(np.arange(32, dtype=np.uint8) % 16, (256, 1))
+    scale = np.arange(256, dtype=np.uint8)[:, None]
+    got = ops.npu_mx_dequant(dev(ref.pack(code)), dev(scale), dst_type=dtype).cpu()
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(ref.values(code, scale).astype(np.float32)).to(dtype)
+    assert torch.equal(got.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0)) and torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(torch.signbit(got[:255]), torch.signbit(want[:255]))
+
+
+# ------------------------------------------------------------------------------------------------ norm
+def norm_ref(x1, x2, gamma, beta, eps):
+    x = x1 if x2 is None else (x1.float() + x2.float()).to(x1.dtype)
+    v = x.double().numpy()
+    y = v * (1.0 / np.sqrt((v * v).mean(-1, keepdims=True) + eps)) * gamma.double().numpy()
+    if beta is not None:
+        y = y + beta.double().numpy()
+    return x, ref.rounded(y, x1.dtype)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("rows,cols,residual,bias,wide", [
+    (1, 32, True, False, False), (3, 96, False, True, False), (5, 1024, True, True, True), (777, 2048, True, False, False),
+    (2, 7168, True, False, True), (4, 8192, False, False, False), (3, 8224, True, True, False), (2, 16384, True, False, False),
+    (2, 16416, True, True, False), (3, 40960, False, False, True)])
+def test_norm_with_every_kind_of_output(K, dtype, rows, cols, residual, bias, wide):
+    say("norm", dtype, rows, cols, residual, bias, wide)
+    g = torch.Generator().manual_seed(rows + cols)
+    x1 = (torch.randn(rows, cols, generator=g) * 3).to(dtype)
+    x2 = torch.randn(rows, cols, generator=g).to(dtype) if residual else None
+    kind = torch.float32 if wide else dtype
+    gamma = (1 + 0.2 * torch.randn(cols, generator=g)).to(kind)
+    beta = (0.1 * torch.randn(cols, generator=g)).to(kind) if bias else None
+    x, y = norm_ref(x1, x2, gamma, beta, 1e-6)
+    on = [None if t is None else t.to(DEV) for t in (x1, x2, gamma, beta)]
+    for to in (K.NORM_INT8, K.NORM_MXFP4, K.NORM_PLAIN):
+        q, scale, got_y, got_x = K.add_rms_norm_quant(*on, 1e-6, to)
+        assert same_bits(got_x, x) and same_bits(got_y, y)
+        if to == K.NORM_INT8:  # what the token quantiser of the framework makes of y
+            want_q, want_scale = K.dynamic_quant(got_y)
+            assert torch.equal(q, want_q) and torch.equal(scale, want_scale)
+        elif to == K.NORM_MXFP4:
+            want_q, want_scale = ref.quantise(y.double().numpy())
+            assert np.array_equal(q.cpu().numpy(), ref.pack(want_q)) and np.array_equal(scale.cpu().numpy(), want_scale)
+        else:
+            assert q is None and scale is None
+
+
+@pytest.mark.parametrize("cols", [8, 40, 1000, 8200, 20488])
+def test_norm_to_int8_of_odd_widths(ops, K, cols):
+    say("norm int8", cols)
+    g = torch.Generator().manual_seed(cols)
+    x1, x2 = (torch.randn(7, cols, generator=g).to(torch.bfloat16) for _ in range(2))
+    gamma = torch.rand(cols, generator=g).to(torch.bfloat16)
+    x1[3], x2[3] = 0, 0      # a row of zeros
+    x1[4, 0] = float("nan")  # and rows that are not numbers
+    x1[5, 1] = float("inf")
+    q, scale, y, x = ops.npu_add_rms_norm_dynamic_quant(x1.to(DEV), x2.to(DEV), gamma.to(DEV))
+    keep = [0, 1, 2, 3, 6]
+    want_x, want_y = norm_ref(x1[keep], x2[keep], gamma, None, 1e-6)
+    assert same_bits(x[keep], want_x) and same_bits(y[keep], want_y)
+    assert y[4].isnan().all() and y[5, 1].isnan()
+    want_q, want_scale = K.dynamic_quant(y)
+    assert torch.equal(q, want_q) and torch.equal(scale.nan_to_num(nan=-1.0), want_scale.nan_to_num(nan=-1.0))
+    assert not q[3].any() and scale[3] == 0
+
+
+@pytest.mark.parametrize("cols", [7168, 16384, 20480])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_norm_in_place(K, cols, kind):
+    """The sum may be written over either of its operands."""
+    from vllm_ascend_amd import _lib
+
+    say("norm in place", cols, kind)
+    g = torch.Generator().manual_seed(cols)
+    x1, x2 = (torch.randn(3, cols, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    gamma = torch.rand(cols, generator=g).to(torch.bfloat16).to(DEV)
+    q, scale, y, x = K.add_rms_norm_quant(x1, x2, gamma, None, 1e-6, kind)
+    for over in (0, 1):
+        a, b = x1.clone(), x2.clone()
+        q2, scale2, y2 = torch.empty_like(q), torch.empty_like(scale), torch.empty_like(y)
+        _lib.check(_lib.load().moe355_add_rms_norm_quant(
+            a.data_ptr(), b.data_ptr(), gamma.data_ptr(), None, 1, 1, 3, cols, 1e-6, kind, (a, b)[over].data_ptr(),
+            y2.data_ptr(), q2.data_ptr(), scale2.data_ptr(), torch.cuda.current_stream().cuda_stream), "norm")
+        assert torch.equal((a, b)[over], x) and torch.equal(y2, y) and torch.equal(q2, q) and torch.equal(scale2, scale)
+
+
+# ------------------------------------------------------------------------------------------------ products
+def counts_of(rng, E, rows, kind):
+    if kind == "even":
+        return np.bincount(np.arange(rows) % E, minlength=E)
+    if kind == "one":  # all rows at the last expert but one, the others empty
+        c = np.zeros(E, dtype=np.int64)
+        c[max(E - 2, 0)] = rows
+        return c
+    p = 1.0 / np.arange(1, E + 1) ** 1.1
+    return np.bincount(rng.choice(E, rows, p=rng.permutation(p / p.sum())), minlength=E)
+
+
+PRODUCTS = [
+    # E, N, K, rows, how they are spread
+    (1, 64, 64, 1, "even"), (1, 64, 128, 33, "even"), (3, 128, 192, 7, "zipf"), (4, 64, 256, 64, "one"),
+    (5, 192, 320, 100, "zipf"), (8, 2816, 1024, 64, "zipf"), (8, 1024, 1408, 130, "even"), (128, 1536, 2048, 512, "zipf"),
+    (16, 128, 7168, 32, "zipf"), (2, 256, 704, 300, "zipf"), (7, 320, 448, 700, "zipf"), (1, 512, 512, 1000, "even"),
+    (3, 1088, 576, 1900, "zipf"), (300, 64, 64, 900, "zipf"), (2, 4096, 512, 5, "one"), (1, 320, 1024, 257, "even"),
+    (4, 704, 960, 2100, "zipf"),
+]
+
+
+def make_product(E, N, Kd, rows, kind, seed=0, spread=2, tokens=None, heavy=False):
+    rng = np.random.default_rng(seed + E * 1000 + N + Kd + rows)
+    counts = counts_of(rng, E, rows, kind)
+    row_token = None if tokens is None else rng.integers(0, tokens, rows).astype(np.int32)
+    xc, xs = ref.random_mx(rng, (rows if tokens is None else tokens, Kd), spread, heavy)
+    wc, ws = ref.random_mx(rng, (E, N, Kd), spread)
+    ws = ws - 5  # weights of about 0.03
+    return rng, counts, row_token, xc, xs, wc, ws
+
+
+@pytest.mark.parametrize("case", PRODUCTS, ids=str)
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+def test_product_to_16_bits(ops, case, dtype):
+    say("gmm_mx", case, dtype)
+    _, counts, _, xc, xs, wc, ws = make_product(*case, heavy=True)
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    want = ref.rounded(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts), dtype)
+    for list_type, group_list in ((1, counts), (0, counts.cumsum())):
+        out = ops.npu_grouped_matmul([dev(ref.pack(xc))], [w], scale=[s], per_token_scale=[dev(xs)],
+                                     group_list=dev(group_list.astype(np.int64)), split_item=2, group_type=0,
+                                     group_list_type=list_type, output_dtype=dtype)[0]
+        assert out.dtype == dtype and same_bits(out, want)
+
+
+@pytest.mark.parametrize("case", PRODUCTS, ids=str)
+@pytest.mark.parametrize("limit", [0.0, 0.75])
+def test_product_with_swiglu(ops, case, limit):
+    """Codes and scales are those of the formula in 64 bits, next to the borders between two codes as well."""
+    say("gmm_mx_swiglu_quant", case, limit)
+    tokens = max(1, case[3] // 3)
+    _, counts, row_token, xc, xs, wc, ws = make_product(*case, seed=1, tokens=tokens)
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    codes, scale = ops.npu_grouped_matmul_swiglu_quant_v2(
+        dev(ref.pack(xc)), [w], [s], dev(xs), dev(counts.astype(np.int64)), group_list_type=1, swiglu_limit=limit,
+        row_map=dev(row_token))
+    y = ref.swiglu(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts, row_token), limit)
+    c, sc = ref.quantise(y)
+    assert np.array_equal(scale.cpu().numpy(), sc) and np.array_equal(codes.cpu().numpy(), ref.pack(c))
+
+
+@pytest.mark.parametrize("rows", [40, 700])
+def test_rows_that_no_group_has_stay_as_they_were(K, rows):
+    from vllm_ascend_amd import _lib
+
+    say("rows outside the groups", rows)
+    E, N, Kd = 5, 192, 320
+    _, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "zipf")
+    counts = np.maximum(counts - 3, 0)
+    used = int(counts.sum())
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    x, x_scale, lib = dev(ref.pack(xc)), dev(xs), _lib.load()
+    n = lib.moe355_gmm_mx_workspace(rows, N, Kd, E)
+    space = torch.empty(n, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    want = ref.rounded(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)[:used], torch.bfloat16)
+    for list_type, gl in ((1, counts), (0, counts.cumsum())):
+        gl = dev(gl.astype(np.int64))
+        out = torch.full((rows, N), 7.0, dtype=torch.bfloat16, device=DEV)
+        _lib.check(lib.moe355_gmm_mx(x.data_ptr(), x_scale.data_ptr(), None, rows, w.data_ptr(), s.data_ptr(), gl.data_ptr(),
+                                     list_type, rows, Kd, N, E, out.data_ptr(), 1, space.data_ptr(), n, stream), "gmm_mx")
+        assert same_bits(out[:used], want) and (out[used:] == 7.0).all()
+        codes = torch.full((rows, N // 4), 9, dtype=torch.uint8, device=DEV)
+        scale = torch.full((rows, N // 64), 9, dtype=torch.uint8, device=DEV)
+        _lib.check(lib.moe355_gmm_mx_swiglu_quant(
+            x.data_ptr(), x_scale.data_ptr(), None, rows, w.data_ptr(), s.data_ptr(), gl.data_ptr(), list_type, rows, Kd, N, E,
+            0.0, codes.data_ptr(), scale.data_ptr(), space.data_ptr(), n, stream), "gmm_mx_swiglu_quant")
+        assert (codes[used:] == 9).all() and (scale[used:] == 9).all()
+        y = ref.swiglu(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)[:used])
+        c, sc = ref.quantise(y)
+        assert np.array_equal(codes[:used].cpu().numpy(), ref.pack(c)) and np.array_equal(scale[:used].cpu().numpy(), sc)
+
+
+@pytest.mark.parametrize("rows", [40, 700])
+def test_group_lists_that_ask_for_more_than_there_is(ops, rows):
+    """Counts past the last row, negative ones, sums that go back: rows are cut to those that exist, none is written twice by
+    two experts of a list of counts, and nothing outside is read or written."""
+    say("group lists out of range", rows)
+    E, N, Kd = 4, 64, 128
+    _, _, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    x, x_scale = dev(ref.pack(xc)), dev(xs)
+    half = rows // 2
+    for list_type, gl, counts in (
+            (1, [half, 10 * rows, 5, 1 << 40], [half, rows - half, 0, 0]),
+            (1, [-4, half, -1, rows], [0, half, 0, rows - half]),
+            (0, [half, half, 1 << 50, 1 << 50], [half, 0, rows - half, 0])):
+        out = ops.npu_grouped_matmul([x], [w], scale=[s], per_token_scale=[x_scale], group_list=torch.tensor(gl, device=DEV),
+                                     split_item=2, group_type=0, group_list_type=list_type)[0]
+        assert same_bits(out, ref.rounded(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts), torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows", [9, 600])
+def test_row_map_with_rows_that_are_not_there(ops, rows):
+    """An index outside the rows counts as a row of zeros; the same index may come any number of times."""
+    say("row map out of range", rows)
+    E, N, Kd, tokens = 2, 128, 192, 5
+    _, counts, row_token, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even", tokens=tokens)
+    row_token[::4] = [-1, tokens, 2**31 - 1, -(2**31)][: len(row_token[::4])] if rows < 16 else -1
+    row_token[1::4] = 3
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    codes, scale = ops.npu_grouped_matmul_swiglu_quant_v2(
+        dev(ref.pack(xc)), w, s, dev(xs), dev(counts.astype(np.int64)), group_list_type=1, row_map=dev(row_token))
+    c, sc = ref.quantise(ref.swiglu(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts, row_token)))
+    assert np.array_equal(codes.cpu().numpy(), ref.pack(c)) and np.array_equal(scale.cpu().numpy(), sc)
+
+
+@pytest.mark.parametrize("rows", [6, 600])
+def test_scales_that_stand_for_nan_and_far_powers(ops, rows):
+    """A block without a value makes its row's results NaN and no other row's; powers of two at the ends of fp32 hold."""
+    say("special scales", rows)
+    E, N, Kd = 2, 64, 128
+    rng, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    xs[0], xs[1], xs[2] = 255, 0, 250  # NaN; 2^-127, a weight's 2^-8 on top: below fp32; 2^123
+    xs[3, 1] = 255
+    wc[0, 5, :32] = 0
+    ws[0, 5, 0], ws[:, 7] = 255, 0
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    out = ops.npu_grouped_matmul([dev(ref.pack(xc))], [w], scale=[s], per_token_scale=[dev(xs)],
+                                 group_list=dev(counts.astype(np.int64)), split_item=2, group_type=0, group_list_type=1)[0]
+    out = out.cpu().double().numpy()
+    x, wv = ref.values(xc, xs), ref.values(wc, ws)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want = ref.rounded(ref.products(x, wv, counts), torch.bfloat16).double().numpy()
+    assert np.array_equal(np.isnan(out), np.isnan(want))
+    # results below the smallest normal number may be zero
+    keep = ~np.isnan(want) & ((np.abs(want) >= 2.0 ** -126) | (want == 0))
+    assert np.array_equal(out[keep], want[keep])
+    assert (np.abs(out[~keep & ~np.isnan(want)]) < 2.0 ** -125).all()
+
+
+@pytest.mark.parametrize("rows", [20, 600])
+def test_swiglu_of_gates_far_from_zero(ops, rows):
+    """Gates below the range of a 32-bit exponential, results that overflow, results of zero."""
+    say("far gates", rows)
+    E, N, Kd = 2, 128, 64
+    rng, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even", spread=0)
+    for i, p in enumerate([0, 3, 4, 5, 6, 8, 40, 60, 70]):
+        xs[i::9] = 127 + p
+    xc[4] = 0
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc)), dev(ws + 5))
+    codes, scale = ops.npu_grouped_matmul_swiglu_quant_v2(
+        dev(ref.pack(xc)), w, s, dev(xs), dev(counts.astype(np.int64)), group_list_type=1)
+    with np.errstate(over="ignore", invalid="ignore"):
+        c, sc = ref.quantise(ref.swiglu(ref.products(ref.values(xc, xs), ref.values(wc, ws + 5), counts)))
+    assert np.array_equal(scale.cpu().numpy(), sc)
+    c[np.repeat(sc == 0, 32, -1)] = 0  # blocks at the smallest scale: subnormal values
+    got = ref.unpack(codes.cpu().numpy())
+    got[np.repeat(sc == 0, 32, -1)] = 0
+    assert np.array_equal(got, c)
+
+
+@pytest.mark.parametrize("rows,N,Kd", [(1, 32, 64), (5, 96, 320), (130, 4096, 7168), (1000, 672, 1408)])
+def test_dense_product(ops, rows, N, Kd):
+    say("dense", rows, N, Kd)
+    _, _, _, xc, xs, wc, ws = make_product(1, N, Kd, rows, "even")
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc[0])), dev(ws[0]))
+    out = ops.npu_quant_matmul(dev(ref.pack(xc)), w, s, pertoken_scale=dev(xs), output_dtype=torch.float16)
+    assert same_bits(out, ref.rounded(ref.values(xc, xs) @ ref.values(wc, ws)[0].T, torch.float16))
+    lead = ops.npu_quant_matmul(dev(ref.pack(xc))[None], w, s, pertoken_scale=dev(xs)[None], output_dtype=torch.float16)
+    assert lead.shape == (1, rows, N) and torch.equal(lead[0], out)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def build(E, k, H, I, dtype=torch.bfloat16, seed=0, shared=None, **layer_kw):
+    from vllm_ascend_amd.fused_moe.contracts import FusedMoEConfig
+    from vllm_ascend_amd.fused_moe.layer import AscendRoutedExperts
+    from vllm_ascend_amd.fused_moe.router import AscendFusedTopKRouter
+    from vllm_ascend_amd.quantization import get_scheme_class
+
+    rng = np.random.default_rng(seed)
+    w13, s13 = ref.random_mx(rng, (E, 2 * I, H), 1)
+    w2, s2 = ref.random_mx(rng, (E, H, I), 1)
+    s13, s2 = s13 - 5, s2 - 5
+    layer = AscendRoutedExperts(
+        FusedMoEConfig(num_experts=E, experts_per_token=k, hidden_dim=H, intermediate_size_per_partition=I),
+        get_scheme_class("W4A4_MXFP4", "moe")(in_dtype=dtype), AscendFusedTopKRouter(k, E, renormalize=True), device=DEV,
+        shared_experts=shared, **layer_kw)
+    layer.load_weights({"w13_weight": torch.from_numpy(ref.pack(w13)), "w13_weight_scale": torch.from_numpy(s13),
+                        "w2_weight": torch.from_numpy(ref.pack(w2)), "w2_weight_scale": torch.from_numpy(s2)})
+    return layer, ref.values(w13, s13), ref.values(w2, s2)
+
+
+def experts_ref(y, ids, weights, w13, w2, dtype, residual=None):
+    """The layer of hidden states y, expert by expert in 64 bits, rounded where the path rounds."""
+    T, k = ids.shape
+    order = np.argsort(ids.reshape(-1), kind="stable")
+    counts = np.bincount(ids.reshape(-1), minlength=len(w13))
+    x = ref.values(*ref.quantise(y.double().cpu().numpy()))[order // k]
+    h = ref.values(*ref.quantise(ref.swiglu(ref.products(x, w13, counts))))
+    o = ref.rounded(ref.products(h, w2, counts), dtype).double().numpy()
+    pairs = np.empty_like(o)
+    pairs[order] = o
+    out = (pairs.reshape(T, k, -1) * weights.double().cpu().numpy()[:, :, None]).sum(1)
+    return out if residual is None else out + residual
+
+
+def close(got, want, dtype, k):
+    """One rounding to 16 bits (half a step) and k additions in 32 bits: 2^-8 or 2^-11 of the value plus k 2^-24 of the terms'
+    size, for which the row's largest value times sqrt(k) stands."""
+    got = got.double().cpu().numpy()
+    bound = np.abs(want) * torch.finfo(dtype).eps / 2 * 1.001 + k * 2.0 ** -24 * np.abs(want).max(-1, keepdims=True) * 4
+    return bool((np.abs(got - want) <= bound).all())
+
+
+@pytest.mark.parametrize("T,E,k,H,I,dtype", [
+    (1, 8, 2, 256, 192, torch.bfloat16), (5, 8, 2, 1024, 1408, torch.float16), (64, 60, 4, 448, 128, torch.bfloat16),
+    (300, 16, 8, 512, 320, torch.bfloat16), (700, 4, 2, 576, 704, torch.float16)])
+def test_norm_and_layer_together(ops, T, E, k, H, I, dtype):
+    """Residual addition and norm, the router on the norm's output, the experts on its MXFP4 form."""
+    say("norm and layer", T, E, k, H, I, dtype)
+    layer, w13, w2 = build(E, k, H, I, dtype)
+    g = torch.Generator().manual_seed(T)
+    x1, x2 = (torch.randn(T, H, generator=g).to(dtype).to(DEV) for _ in range(2))
+    gamma = (1 + 0.1 * torch.randn(H, generator=g)).to(dtype).to(DEV)
+    logits = torch.randn(T, E, generator=g).to(DEV)
+    codes, scale, y, x = ops.npu_add_rms_norm_dynamic_quant(x1, x2, gamma, dst_type=torch.float4_e2m1fn_x2)
+    weights, ids = layer.router.select_experts(y, logits)
+    want = experts_ref(y, ids.cpu().numpy(), weights, w13, w2, dtype)
+    out = layer(y, logits)
+    assert out.shape == y.shape and out.dtype == dtype and close(out, want, dtype, k)
+    layer.ascend_pertoken_scale = scale  # the rows as the norm has quantised them
+    assert torch.equal(layer(codes, logits), out)
+    res = layer.forward_impl(codes, logits)
+    assert torch.equal(res.expert_tokens.cpu(), torch.bincount(ids.flatten().cpu().long(), minlength=E))
+
+
+def test_layer_with_a_shared_expert(ops):
+    from vllm_ascend_amd.fused_moe.shared_experts import AscendSharedExperts
+
+    say("layer with a shared expert")
+    T, E, k, H, I = 33, 8, 2, 256, 128
+    g = torch.Generator().manual_seed(2)
+    up = torch.randint(-127, 128, (2 * I, H), generator=g, dtype=torch.int8).to(DEV)
+    down = torch.randint(-127, 128, (H, I), generator=g, dtype=torch.int8).to(DEV)
+    su, sd = (torch.rand(n, generator=g).to(DEV) * 1e-3 for n in (2 * I, H))
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(T, E, generator=g).to(DEV)
+    for overlap in (False, True):
+        shared = AscendSharedExperts(up, su, down, sd, multistream_overlap=overlap)
+        layer, w13, w2 = build(E, k, H, I, shared=shared)
+        weights, ids = layer.router.select_experts(x, logits)
+        extra = shared(x)
+        shared.wait()
+        want = experts_ref(x, ids.cpu().numpy(), weights, w13, w2, torch.bfloat16, extra.double().cpu().numpy())
+        assert close(layer(x, logits), want, torch.bfloat16, k + 1)
+
+
+def test_int8_layer_on_rows_that_the_norm_quantised(ops):
+    """The norm's int8 rows and the 16-bit ones give the W8A8 layer the same bits."""
+    from _inputs import CONFIGS, make_layer
+    from _layer_utils import build_layer
+
+    say("int8 layer behind the norm")
+    cfg = CONFIGS["c2_small"]
+    layer = build_layer(cfg, make_layer(cfg, seed=0), DEV)
+    g = torch.Generator().manual_seed(3)
+    x1, x2 = (torch.randn(cfg.T, cfg.H, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    gamma = (1 + 0.1 * torch.randn(cfg.H, generator=g)).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(cfg.T, cfg.E, generator=g).to(DEV)
+    q, scale, y, _ = ops.npu_add_rms_norm_dynamic_quant(x1, x2, gamma)
+    want = layer(y, logits)
+    layer.ascend_pertoken_scale = scale
+    assert torch.equal(layer(q, logits), want)
+
+
+@pytest.mark.parametrize("T", [4, 400])
+def test_captured_and_replayed(ops, T):
+    """Norm and layer in a graph, replayed on other inputs with eager calls between."""
+    say("graph", T)
+    E, k, H, I = 8, 2, 512, 256
+    layer, _, _ = build(E, k, H, I)
+    g = torch.Generator().manual_seed(T)
+    x1, x2 = (torch.empty(T, H, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    logits = torch.empty(T, E, device=DEV)
+    gamma = torch.ones(H, dtype=torch.bfloat16, device=DEV)
+
+    def fill():
+        for t in (x1, x2, logits):
+            t.copy_(torch.randn(t.shape, generator=g))
+
+    def step():
+        codes, scale, y, x = ops.npu_add_rms_norm_dynamic_quant(x1, x2, gamma, dst_type=torch.float4_e2m1fn_x2)
+        weights, ids = layer.router.select_experts(y, logits)
+        return x, layer.quant_method.apply(layer, y, weights, ids).routed_out
+
+    fill()
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs over the same layer
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for i in range(4):
+        fill()
+        for graph, _ in graphs:
+            graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_on_another_stream(ops):
+    say("other stream")
+    layer, _, _ = build(8, 2, 512, 256)
+    g = torch.Generator().manual_seed(5)
+    x, logits = torch.randn(50, 512, generator=g).to(torch.bfloat16).to(DEV), torch.randn(50, 8, generator=g).to(DEV)
+    want = layer(x, logits)
+    torch.cuda.synchronize()
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            outs.append(layer(x, logits))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_layer_of_no_tokens(ops):
+    say("no tokens")
+    layer, _, _ = build(8, 2, 512, 256)
+    out = layer.quant_method.apply(layer, torch.empty(0, 512, dtype=torch.bfloat16, device=DEV),
+                                   torch.empty(0, 2, device=DEV), torch.empty(0, 2, dtype=torch.int32, device=DEV)).routed_out
+    assert out.shape == (0, 512)

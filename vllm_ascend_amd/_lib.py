@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libmoe355.so")
@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libmoe355.so")
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 W_ENK, W_EKN = 0, 1
 GL_CUMSUM, GL_COUNT = 0, 1
+NORM_PLAIN, NORM_INT8, NORM_MXFP4 = 0, 1, 2
 
 ABI_VERSION = 1
 
@@ -132,6 +133,17 @@ PROTOTYPES = {
     "moe355_gmm_tile_rows": (c_int, [c_int64, c_int64, c_int64, c_int]),
     "moe355_token_unpermute": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
                                        c_void_p, c_void_p]),
+    "moe355_dynamic_mx_quant": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "moe355_mx_dequant": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "moe355_add_rms_norm_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_double,
+                                          c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "moe355_format_cast_mx": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "moe355_gmm_mx_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "moe355_gmm_mx": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,
+                              c_int64, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "moe355_gmm_mx_swiglu_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64,
+                                           c_int64, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
+                                           c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,178 @@
+// What the kernels of the MXFP4 products share.
+//
+// An operand of v_mfma_scale_f32_32x32x64_f8f6f4 with 4-bit values is 32 rows x 64 K: lane l holds row l % 32 and 32 values of
+// its K, one block, in 16 bytes, and the block's scale in a byte of a register (which one: an immediate).  Any order of K will
+// do as long as both operands have it, so a window of 256 K is taken as two runs of blocks, one for either half of the lanes:
+// lane l reads blocks 4 (l / 32) .. + 3 of its row, 64 bytes that follow each other, and their scales as one register.  A last
+// window of nb < 4 steps (K = 64 nb) has runs of nb blocks.
+//
+// Weights are kept in that order: [E][N / 32][K / 64] operands of 1 KiB (lane l's 16 bytes at 16 l), scales [E][N / 32][windows]
+// of 256 bytes (lane l's four at 4 l).
+//
+// Channels are the rows of the product and tokens its columns: lane l has token l % 32, and of channels 8 (i / 4) + 4 (l / 32) +
+// i % 4 the i-th of its 16 results; so a block of 32 output channels of a token is in two lanes.
+//
+// Sums are exact in most cases: products are multiples of 2^(sx + sw - 2), and 24 bits hold the sum of thousands of them with
+// scales that lie some powers of two apart.  So the order of K, and its split over wavefronts, hardly ever shows.
+#pragma once
+
+#include "mx_common.h"
+
+namespace moe355 {
+
+struct MxArgs {
+    const uint8_t* x;           // [x_rows, K / 2] codes
+    const uint8_t* x_scale;     // [x_rows, K / 32]
+    const int32_t* row_token;   // sorted row -> row of x, or NULL: the rows of x are sorted
+    const uint8_t* w;           // operands as above
+    const uint8_t* w_scale;
+    const int64_t* group_list;  // NULL: one expert, all rows
+    int gl_type;
+    int64_t rows, x_rows, K, N;
+    int E;
+    float limit;                // SwiGLU's clamp
+    void* out;                  // 16-bit [rows, N], or codes [rows, N / 4] of the N / 2 values of SwiGLU
+    uint8_t* out_scale;         // [rows, N / 64]
+};
+
+enum { MX_HALF = 0, MX_SWIGLU = 1 };
+
+__device__ __forceinline__ v16f mfma_mx(v4i a, v4i b, v16f c, int sa, int sb, int j)
+{
+    const v8i A = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, B = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+    // 4: both operands e2m1; the byte of the scale registers is an immediate
+    switch (j) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 1, sa, 1, sb);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 2, sa, 2, sb);
+    default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 3, sa, 3, sb);
+    }
+}
+
+// Rows [row0, row1) of expert e, inside [0, rows) whatever the list holds.  Every lane of a wavefront calls it.
+__device__ __forceinline__ void mx_expert_rows(const MxArgs& a, int e, int lane, int64_t& row0, int64_t& row1)
+{
+    if (!a.group_list) {
+        row0 = 0;
+        row1 = a.rows;
+    } else if (a.gl_type == MOE355_GL_CUMSUM) {
+        row0 = e > 0 ? a.group_list[e - 1] : 0;
+        row1 = a.group_list[e];
+    } else {
+        int64_t total = 0;
+        for (int i = lane; i < e; i += 64) {
+            const int64_t n = a.group_list[i];
+            total += n < 0 ? 0 : n < a.rows ? n : a.rows;  // at most 2^31 each
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+        row0 = total;
+        const int64_t n = a.group_list[e];
+        row1 = row0 + (n > 0 ? n : 0);
+    }
+    row0 = row0 < 0 ? 0 : row0 > a.rows ? a.rows : row0;
+    row1 = row1 < row0 ? row0 : row1 > a.rows ? a.rows : row1;
+}
+
+// silu(g) u from its definition in 64 bits, rounded once
+__device__ __forceinline__ float swiglu_f64(float g, float u)
+{
+    const double d = (double)g;
+    return (float)(d / (1.0 + exp(-d)) * (double)u);
+}
+
+// 16 values of silu(gate) * up a lane.
+//
+// What is quantised is the value of the formula, rounded to binary32.  m_silu and the product are a few units in the last place
+// off it, which shows in the codes only next to a border: the middles between two codes and the powers of two where the scale
+// changes, all of which have a mantissa of two bits and then zeros.  A value within 16 units of such a number (1.5 in 10^5 of
+// them) is computed again in 64 bits, and so is one whose gate is below -80, where m_silu ends.  The codes are therefore those
+// of the formula whatever exp is used, for 2 instructions a value.
+__device__ __forceinline__ void mx_swiglu(v16f& g, const v16f& up, float limit)
+{
+    v16f u = up;
+    if (limit > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            g[i] = g[i] > limit ? limit : g[i];
+            u[i] = u[i] > limit ? limit : u[i];
+            u[i] = u[i] < -limit ? -limit : u[i];
+        }
+    }
+    v16f y;
+    uint32_t near = 0xffffffffu;
+    float least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        y[i] = m_silu(g[i]) * u[i];
+        const uint32_t key = (__float_as_uint(y[i]) << 11) + (16u << 11);
+        near = key < near ? key : near;
+        least = g[i] < least ? g[i] : least;
+    }
+    if (near < (32u << 11) || least < -80.0f) {
+        uint32_t todo = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t key = (__float_as_uint(y[i]) << 11) + (16u << 11);
+            if ((key < (32u << 11) || g[i] < -80.0f) && g[i] != 0.0f && u[i] != 0.0f) todo |= 1u << i;
+        }
+        while (todo) {
+            const int at = __builtin_ctz(todo);
+            todo &= todo - 1;
+            float gi = g[0], ui = u[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) gi = i == at ? g[i] : gi, ui = i == at ? u[i] : ui;
+            const float v = swiglu_f64(gi, ui);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = i == at ? v : y[i];
+        }
+    }
+    g = y;
+}
+
+// A block of 32 channels of a token (this lane's 16 of them in y) to MXFP4: codes 16 bytes at `codes`, its scale at `scale`.
+// Both halves of the wavefront call it together; `store`: whether the lane's token exists.
+__device__ __forceinline__ void mx_store_block(const v16f& y, int half, bool store, uint8_t* codes, uint8_t* scale)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max_u32(m, __float_as_uint(y[i]) & 0x7fffffffu);
+    const v2u both = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    const MxScale s = mx_scale(max_u32(both[0], both[1]));
+    float v[2][8];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = y[i] * s.inverse;
+    // 16 codes: channels 0-3, 8-11 (+ 4 in the upper half) and 16-19, 24-27
+    const uint32_t low = s.finite ? mx_codes8(v[0]) : 0, high = s.finite ? mx_codes8(v[1]) : 0;
+    // lower half: channels 0-15 of the block, upper half: 16-31
+    const v2u p = __builtin_amdgcn_permlane32_swap(low, high, false, false);
+    const uint2 q = make_uint2(__builtin_amdgcn_perm(p[1], p[0], 0x05040100), __builtin_amdgcn_perm(p[1], p[0], 0x07060302));
+    if (store) {
+        *(uint2*)(codes + 8 * half) = q;
+        if (half == 0) *scale = (uint8_t)s.byte;
+    }
+}
+
+// 32 channels of a token as 16-bit values at `to`
+template <int DT>
+__device__ __forceinline__ void mx_store_half(const v16f& y, int half, bool store, uint16_t* to)
+{
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        uint32_t d[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int i = 8 * p + 4 * q + 2 * k;
+                d[q][k] = (uint32_t)f32_to_half<DT>(y[i]) | (uint32_t)f32_to_half<DT>(y[i + 1]) << 16;
+            }
+        // lower half: channels 16 p .. + 7, upper half: 16 p + 8 .. + 15
+        const v2u s0 = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
+        const v2u s1 = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
+        const v4u v = {s0[0], s1[0], s0[1], s1[1]};
+        if (store) *(v4u*)(to + 16 * p + 8 * half) = v;
+    }
+}
+
+}  // namespace moe355

@@ -10,6 +10,14 @@ from . import npu_ops
 from .custom_ops import enable_custom_op
 
 
+def _fp4(dtype):
+    """The quantised type of an MXFP call: four bits, or None (and int8, the default of the int8 calls) for it."""
+    if dtype in (None, torch.int8):
+        return None
+    npu_ops._require_fp4("MXFP MoE quantization on MI355X", dtype)
+    return dtype
+
+
 class MI355XDeviceAdaptor:
     @staticmethod
     def npu_moe_init_routing(hidden_states, topk_ids, *, scale=None, active_num: int, expert_num: int,
@@ -45,7 +53,10 @@ class MI355XDeviceAdaptor:
     def npu_dynamic_quant(hidden_states, dynamic_scale=None, *, act_quant_type=torch.int8,
                           use_mxfp_quant: bool = False):
         if use_mxfp_quant:
-            raise RuntimeError("MXFP MoE quantization is not available on MI355X in this build.")
+            # MXFP4: codes and E8M0 scales
+            if dynamic_scale is None:
+                return npu_ops.npu_dynamic_mx_quant(hidden_states, dst_type=_fp4(act_quant_type))
+            return hidden_states, dynamic_scale
         if dynamic_scale is None:
             return npu_ops.npu_dynamic_quant(hidden_states, dst_type=torch.int8)
         return hidden_states, dynamic_scale
@@ -57,7 +68,10 @@ class MI355XDeviceAdaptor:
         """``group_list_type`` (not in the reference, whose op only takes a running sum): 1 hands the
         per-expert counts of the dispatcher to the kernel as they are, which saves the cumsum launch."""
         if use_mxfp_quant:
-            raise RuntimeError("MXFP MoE quantization is not available on MI355X in this build.")
+            out, out_scale = npu_ops.npu_grouped_matmul_swiglu_quant_v2(
+                x, weight, weight_scale, x_scale, group_list, bias=bias, quant_dtype=_fp4(act_quant_type),
+                group_list_type=group_list_type, swiglu_limit=swiglu_limit)
+            return out, out_scale, None
         enable_custom_op()
         if group_list_type == 1:
             from . import custom_ops, kernels
@@ -77,7 +91,8 @@ class MI355XDeviceAdaptor:
     def get_quant_gmm2_kwargs(*, input_dtype, act_quant_type=None, weight_quant_type=None, scale_type=None,
                               per_token_scale_type=None, use_bf16: bool = True, use_mxfp_quant: bool = False) -> dict:
         if use_mxfp_quant:
-            raise RuntimeError("MXFP MoE quantization is not available on MI355X in this build.")
+            _fp4(act_quant_type)
+            _fp4(weight_quant_type)
         return {"output_dtype": input_dtype if input_dtype in (torch.bfloat16, torch.float16) else torch.bfloat16}
 
     @classmethod
@@ -87,7 +102,8 @@ class MI355XDeviceAdaptor:
                                 use_mxfp_quant: bool = False, bias=None, fallback_output_dtype=None,
                                 mxfp_quant_dtype=None):
         if use_mxfp_quant:
-            raise RuntimeError("MXFP MoE quantization is not available on MI355X in this build.")
+            _fp4(act_quant_type)
+            fallback_output_dtype = input_dtype if input_dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
         if fallback_output_dtype is None:
             first = weight_scale[0] if isinstance(weight_scale, list) else weight_scale
             fallback_output_dtype = first.dtype

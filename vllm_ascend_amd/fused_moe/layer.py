@@ -78,6 +78,8 @@ class AscendRoutedExperts(torch.nn.Module):
         post-load processing (format cast, scale reshapes)."""
         for name, t in tensors.items():
             p = getattr(self, name)
+            if p.dtype == torch.uint8 and t.dtype.is_floating_point and t.element_size() == 1:
+                t = t.view(torch.uint8)  # MXFP4 codes or E8M0 scales under the name of their type: the bytes, not the numbers
             p.data.copy_(t.reshape(p.data.shape).to(p.data.dtype))
         self.quant_method.process_weights_after_loading(self)
 
@@ -120,10 +122,10 @@ class AscendRoutedExperts(torch.nn.Module):
         if self.use_fused_small_batch and fused is not None and fused(self, hidden_states, router_logits, self.router):
             return self.quant_method.apply_small_batch(self, hidden_states, router_logits, self.router,
                                                        self.shared_experts, None)
-        # int8 hidden states = activations the caller quantised (their scales in ascend_pertoken_scale): the
-        # routing weights then take the model dtype of the scheme
+        # int8 hidden states (uint8: MXFP4 codes) = activations the caller quantised (their scales in
+        # ascend_pertoken_scale): the routing weights then take the model dtype of the scheme
         weights_dtype = None
-        if hidden_states.dtype == torch.int8:
+        if hidden_states.dtype in (torch.int8, torch.uint8):
             weights_dtype = getattr(self.quant_method, "in_dtype", torch.bfloat16)
         topk_weights, topk_ids = self.router.select_experts(
             hidden_states, router_logits, enable_force_load_balance=self.enable_force_load_balance,

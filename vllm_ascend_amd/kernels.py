@@ -7,7 +7,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import DT_BF16, DT_F16, DT_F32, GL_COUNT, GL_CUMSUM, W_EKN, W_ENK, check
+from ._lib import (DT_BF16, DT_F16, DT_F32, GL_COUNT, GL_CUMSUM, NORM_INT8, NORM_MXFP4, NORM_PLAIN, W_EKN, W_ENK,
+                   check)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 
@@ -845,3 +846,195 @@ def w4_offset_correction(weight_nz4, weight_scale, group_size, n, k):
     check(lib.moe355_w4_offset_correction(_ptr(w), _ptr(_dev(weight_scale, "weight_scale")), group_size, E, n, k,
                                           _ptr(corr), _stream(w)), "moe355_w4_offset_correction")
     return corr
+
+
+# ---------------------------------------------------------------------- MXFP4
+MX_BLOCK = 32  # values that share a scale
+
+
+def _bytes(t: torch.Tensor, name: str, kinds=("float4_e2m1fn_x2",)) -> torch.Tensor:
+    """Codes or E8M0 scales as uint8, under whichever of their names they come."""
+    if t.dtype == torch.uint8:
+        return t
+    if any(t.dtype == getattr(torch, kind, None) for kind in kinds):
+        return t.view(torch.uint8)
+    raise TypeError(f"{name}: uint8 or {' or '.join(kinds)} tensor expected but got {t.dtype}")
+
+
+def _scale_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
+    return _bytes(t, name, ("float8_e8m0fnu",))
+
+
+def _flat(t: torch.Tensor, name: str, alignment: int = 16) -> torch.Tensor:
+    """Contiguous, on the GPU, and starting where the kernels' wide loads may start (a view into another tensor need not)."""
+    t = _dev(t, name)
+    return t if t.data_ptr() % alignment == 0 else t.clone()
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """An entry point of the library on torch's current stream of a device, which need not be the current device."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, _raw_stream(device.index)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _raw_stream(device.index)), name)
+
+
+def _on(x: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{name} is on {t.device}, the rows on {x.device}")
+
+
+def _rows_of(x: torch.Tensor, op: str, multiple: int) -> tuple[int, int]:
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % multiple:
+        raise ValueError(f"{op}: rows must hold a multiple of {multiple} values, got {tuple(x.shape)}")
+    return x.numel() // x.shape[-1], x.shape[-1]
+
+
+def dynamic_mx_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 / fp16 / fp32 [..., K] -> (codes uint8 [..., K / 2], E8M0 scales uint8 [..., K / 32])."""
+    dt = _dt(x, "x")
+    rows, cols = _rows_of(x, "dynamic_mx_quant", MX_BLOCK)
+    x = _flat(x, "x")
+    codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((*x.shape[:-1], cols // MX_BLOCK), dtype=torch.uint8, device=x.device)
+    _call(x.device, "moe355_dynamic_mx_quant", _ptr(x), dt, rows, cols, _ptr(codes), _ptr(scale))
+    return codes, scale
+
+
+def mx_dequant(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [..., K] that codes [..., K / 2] and scales [..., K / 32] stand for."""
+    if dtype not in _DT:
+        raise TypeError(f"mx_dequant: float16, float32 or bfloat16 output expected but got {dtype}")
+    codes, scale = _bytes(codes, "codes"), _scale_bytes(scale, "scale")
+    rows, half = _rows_of(codes, "mx_dequant", MX_BLOCK // 2)
+    if scale.shape != (*codes.shape[:-1], half * 2 // MX_BLOCK):
+        raise ValueError(f"mx_dequant: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
+    codes, scale = _flat(codes, "codes", 4), _dev(scale, "scale")
+    _on(codes, scale=scale)
+    out = torch.empty((*codes.shape[:-1], half * 2), dtype=dtype, device=codes.device)
+    _call(codes.device, "moe355_mx_dequant", _ptr(codes), _ptr(scale), rows, half * 2, _ptr(out), _DT[dtype])
+    return out
+
+
+def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
+    """x = x1 (+ x2), y = RMS norm of x, q and scale = y quantised: int8 with an fp32 scale a row (``NORM_INT8``), MXFP4
+    (``NORM_MXFP4``) or not at all (``NORM_PLAIN``: None, None).  -> (q, scale, y, x); without x2, x is x1 itself."""
+    op = "add_rms_norm_quant"
+    dt = _dt(x1, "x1")
+    _half_dtype(x1.dtype)
+    rows, cols = _rows_of(x1, op, MX_BLOCK if kind == NORM_MXFP4 else 8)
+    if x2 is not None and (x2.shape != x1.shape or x2.dtype != x1.dtype):
+        raise ValueError(f"{op}: x2 {tuple(x2.shape)} {x2.dtype} does not match x1 {tuple(x1.shape)} {x1.dtype}")
+    if gamma.dtype not in (x1.dtype, torch.float32) or gamma.shape != (cols,):
+        raise ValueError(f"{op}: gamma must hold {cols} values of {x1.dtype} or float32, got {tuple(gamma.shape)} "
+                         f"{gamma.dtype}")
+    if beta is not None and (beta.dtype != gamma.dtype or beta.shape != gamma.shape):
+        raise ValueError(f"{op}: beta {tuple(beta.shape)} {beta.dtype} does not match gamma {tuple(gamma.shape)} "
+                         f"{gamma.dtype}")
+    given = x1
+    x1 = _flat(x1, "x1")
+    x2 = None if x2 is None else _flat(x2, "x2")
+    gamma, beta = _flat(gamma, "gamma"), None if beta is None else _flat(beta, "beta")
+    _on(x1, x2=x2, gamma=gamma, beta=beta)
+    dev, lead = x1.device, x1.shape[:-1]
+    y = torch.empty_like(x1)
+    x = torch.empty_like(x1) if x2 is not None else None
+    q = scale = None
+    if kind == NORM_INT8:
+        q = torch.empty(x1.shape, dtype=torch.int8, device=dev)
+        scale = torch.empty(lead, dtype=torch.float32, device=dev)
+    elif kind == NORM_MXFP4:
+        q = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
+        scale = torch.empty((*lead, cols // MX_BLOCK), dtype=torch.uint8, device=dev)
+    _call(dev, "moe355_add_rms_norm_quant", _ptr(x1), _ptr(x2), _ptr(gamma), _ptr(beta), dt, _dt(gamma, "gamma"), rows,
+          cols, float(epsilon), kind, _ptr(x), _ptr(y), _ptr(q), _ptr(scale))
+    return q, scale, y, given if x is None else x
+
+
+def mx_scale_columns(k: int) -> int:
+    """Bytes of scales a channel in the storage of the products: 8 for every 256 values, whole windows."""
+    return (k + 255) // 256 * 8
+
+
+def format_cast_mx(codes: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights [E, N, K / 2] and scales [E, N, K / 32] -> the storage of the products: the same shape, and
+    [E, N, ceil(K / 256) * 8]."""
+    codes, scale = _bytes(codes, "weight"), _scale_bytes(scale, "scale")
+    if codes.dim() != 3 or scale.dim() != 3:
+        raise TypeError("format_cast_mx expects 3-D codes and scales")
+    E, n, k = codes.shape[0], codes.shape[1], codes.shape[2] * 2
+    if n % 32 or k % 64 or not codes.numel():
+        raise ValueError(f"format_cast_mx: N must be a multiple of 32 and K of 64, got E = {E}, N = {n}, K = {k}")
+    if scale.shape != (E, n, k // MX_BLOCK):
+        raise ValueError(f"format_cast_mx: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
+    codes, scale = _flat(codes, "weight"), _dev(scale, "scale")
+    _on(codes, scale=scale)
+    out = torch.empty_like(codes)
+    out_scale = torch.empty((E, n, mx_scale_columns(k)), dtype=torch.uint8, device=codes.device)
+    _call(codes.device, "moe355_format_cast_mx", _ptr(codes), _ptr(scale), E, n, k, _ptr(out), _ptr(out_scale))
+    return out, out_scale
+
+
+def _mx_operands(op, x, x_scale, weight, weight_scale, group_list, row_map, n_multiple):
+    """The checks of the products; -> contiguous operands and (rows, n, k, E)."""
+    x, x_scale = _bytes(x, "x"), _scale_bytes(x_scale, "x_scale")
+    weight, weight_scale = _bytes(weight, "weight"), _scale_bytes(weight_scale, "weight_scale")
+    if weight.dim() != 3:
+        raise ValueError(f"{op}: weight must be [E, N, K / 2] (format_cast_mx), got {tuple(weight.shape)}")
+    E, n, k = weight.shape[0], weight.shape[1], weight.shape[2] * 2
+    if n % n_multiple or k % 64 or not weight.numel():
+        raise ValueError(f"{op}: N must be a multiple of {n_multiple} and K of 64, got E = {E}, N = {n}, K = {k}")
+    if weight_scale.shape != (E, n, mx_scale_columns(k)):
+        raise ValueError(f"{op}: weight_scale must be {(E, n, mx_scale_columns(k))} (format_cast_mx), got "
+                         f"{tuple(weight_scale.shape)}")
+    if x.dim() != 2 or x.shape[1] * 2 != k:
+        raise ValueError(f"{op}: x must be [rows, K / 2 = {k // 2}], got {tuple(x.shape)}")
+    if x_scale.shape != (x.shape[0], k // MX_BLOCK):
+        raise ValueError(f"{op}: x_scale must be {(x.shape[0], k // MX_BLOCK)}, got {tuple(x_scale.shape)}")
+    if group_list is None:
+        if E != 1:
+            raise ValueError(f"{op}: {E} experts need a group_list")
+    elif group_list.dim() != 1 or group_list.numel() != E or group_list.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{op}: group_list must hold one integer per expert ({E}), got {tuple(group_list.shape)} "
+                         f"{group_list.dtype}")
+    rows = x.shape[0]
+    if row_map is not None:
+        if row_map.dtype != torch.int32 or row_map.dim() != 1:
+            raise TypeError(f"{op}: row_map must be a vector of int32, got {tuple(row_map.shape)} {row_map.dtype}")
+        rows, row_map = row_map.numel(), _dev(row_map, "row_map")
+    x, x_scale = _flat(x, "x"), _dev(x_scale, "x_scale")
+    weight, weight_scale = _flat(weight, "weight"), _flat(weight_scale, "weight_scale")
+    group_list = None if group_list is None else _gl(group_list)
+    _on(x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, row_map=row_map)
+    return x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E
+
+
+def gmm_mx(x, x_scale, weight, weight_scale, group_list, group_list_type, out_dtype=torch.bfloat16, row_map=None):
+    """MXFP4 rows [M, K / 2] times their experts' weights [E, N, K / 2] -> 16-bit [rows, N].  row_map: the row of x of every
+    sorted row; without it the rows of x are sorted by expert.  group_list None: one expert, which has all rows."""
+    x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E = _mx_operands(
+        "gmm_mx", x, x_scale, weight, weight_scale, group_list, row_map, 32)
+    out = torch.empty((rows, n), dtype=_half_dtype(out_dtype), device=x.device)
+    lib = _lib.load()
+    ws = _workspace(lib.moe355_gmm_mx_workspace(rows, n, k, E), x.device)
+    _call(x.device, "moe355_gmm_mx", _ptr(x), _ptr(x_scale), _ptr(row_map), x.shape[0], _ptr(weight),
+          _ptr(weight_scale), _ptr(group_list), _gl_type(group_list_type), rows, k, n, E, _ptr(out), _dt(out, "out"),
+          _ptr(ws), ws.numel())
+    return out
+
+
+def gmm_mx_swiglu_quant(x, x_scale, weight, weight_scale, group_list, group_list_type, swiglu_limit=0.0, row_map=None):
+    """... with the gate_up weights [E, 2 I, K / 2], through SwiGLU to MXFP4: (codes [rows, I / 2], scales [rows, I / 32])."""
+    x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E = _mx_operands(
+        "gmm_mx_swiglu_quant", x, x_scale, weight, weight_scale, group_list, row_map, 64)
+    out = torch.empty((rows, n // 4), dtype=torch.uint8, device=x.device)
+    out_scale = torch.empty((rows, n // 64), dtype=torch.uint8, device=x.device)
+    lib = _lib.load()
+    ws = _workspace(lib.moe355_gmm_mx_workspace(rows, n, k, E), x.device)
+    _call(x.device, "moe355_gmm_mx_swiglu_quant", _ptr(x), _ptr(x_scale), _ptr(row_map), x.shape[0], _ptr(weight),
+          _ptr(weight_scale), _ptr(group_list), _gl_type(group_list_type), rows, k, n, E, float(swiglu_limit),
+          _ptr(out), _ptr(out_scale), _ptr(ws), ws.numel())
+    return out, out_scale

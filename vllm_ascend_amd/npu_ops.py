@@ -77,7 +77,10 @@ def npu_grouped_matmul(x, weight, *, bias=None, scale=None, offset=None, antiqua
                        output_dtype=None, tuning_config=None):
     """Quantised grouped matmul, the form the down projection uses: one int8 ``x`` [M, K],
     one tiled weight [E, K, N], per-channel ``scale`` [E, N], ``per_token_scale`` [M],
-    ``group_type=0`` (split along M), ``split_item`` 2 or 3 (single output).  Returns ``[out]``."""
+    ``group_type=0`` (split along M), ``split_item`` 2 or 3 (single output).  Returns ``[out]``.
+
+    MXFP4: ``x`` codes [M, K / 2] with ``per_token_scale`` [M, K / 32], ``weight`` and ``scale`` as
+    :func:`npu_format_cast_mx` returns them."""
     if bias is not None or offset is not None or antiquant_scale is not None or antiquant_offset is not None:
         raise NotImplementedError("npu_grouped_matmul: bias / offset / antiquant operands are not supported")
     if group_type != 0 or split_item not in (2, 3) or act_type != 0:
@@ -100,6 +103,10 @@ def npu_grouped_matmul(x, weight, *, bias=None, scale=None, offset=None, antiqua
     if len(xs) != 1 or len(ws) != 1 or len(ss) != 1 or len(ps) != 1 or ss[0] is None or ps[0] is None:
         raise NotImplementedError("npu_grouped_matmul: expects exactly one x, weight, scale and per_token_scale")
     a, w, s, p = xs[0], ws[0], ss[0], ps[0]
+    if _is_mx(a):
+        if output_dtype not in (None, torch.bfloat16, torch.float16):
+            raise NotImplementedError(f"npu_grouped_matmul: output_dtype {output_dtype} is not supported")
+        return [kernels.gmm_mx(a, p, w, s, group_list, group_list_type, output_dtype or torch.bfloat16)]
     if a.dtype != torch.int8 or w.dtype != torch.int8:
         raise NotImplementedError("npu_grouped_matmul: only the int8 x int8 form is supported")
     if output_dtype not in (None, torch.bfloat16, torch.float16):
@@ -139,7 +146,12 @@ def npu_quant_matmul(x1, x2, scale, *, offset=None, pertoken_scale=None, bias=No
     ``[K, N]`` in the tiled storage of :func:`npu_format_cast`, ``scale`` ``[N]``.
     ``output_dtype=torch.int32``: the raw accumulators (scales ignored, as in the reference call);
     ``output_dtype=torch.bfloat16`` / ``torch.float16``: ``half((acc * pertoken_scale[m]) * scale[n])``.
-    One expert that owns every row: the grouped kernels with E = 1."""
+    One expert that owns every row: the grouped kernels with E = 1.
+
+    MXFP4: ``x1`` codes [M, K / 2] with ``pertoken_scale`` [M, K / 32], ``x2`` [N, K / 2] and ``scale`` as
+    :func:`npu_format_cast_mx` returns them."""
+    if _is_mx(x1):
+        return _mx_quant_matmul(x1, x2, scale, offset, pertoken_scale, bias, output_dtype)
     if offset is not None or bias is not None:
         raise NotImplementedError("npu_quant_matmul: offset / bias are not supported")
     if x1.dtype != torch.int8 or x2.dtype != torch.int8 or x2.dim() != 2:
@@ -172,3 +184,93 @@ def npu_format_cast_int4(packed: torch.Tensor) -> torch.Tensor:
     raw = packed.contiguous().view(torch.uint8).reshape(e, k, n // 2)
     tiled = kernels.format_cast_nz_int4(raw, 1, n, k)
     return tiled.view(packed.dtype).reshape(packed.shape)
+
+
+# ---------------------------------------------------------------------- MXFP4
+def _is_mx(codes: torch.Tensor) -> bool:
+    return codes.dtype == torch.uint8 or codes.dtype == getattr(torch, "float4_e2m1fn_x2", None)
+
+
+def _require_fp4(op: str, dtype) -> None:
+    if dtype not in (None, torch.uint8, getattr(torch, "float4_e2m1fn_x2", torch.uint8)):
+        raise NotImplementedError(f"{op}: {dtype} is not supported (MXFP4: torch.float4_e2m1fn_x2)")
+
+
+def npu_dynamic_mx_quant(x: torch.Tensor, *, axis: int = -1, round_mode: str = "rint", dst_type=None, block_size: int = 32,
+                         scale_alg: int = 0):
+    """bf16 / fp16 / fp32 [..., K] -> MXFP4: (codes uint8 [..., K / 2], two a byte, the first in the low half; E8M0 scales
+    uint8 [..., K / 32])."""
+    _require_fp4("npu_dynamic_mx_quant", dst_type)
+    if axis not in (-1, x.dim() - 1) or block_size != 32 or round_mode != "rint" or scale_alg != 0:
+        raise NotImplementedError("npu_dynamic_mx_quant: blocks of 32 along the last axis, rounded to nearest even, with the "
+                                  "scale of the largest magnitude's exponent (scale_alg=0) only")
+    return kernels.dynamic_mx_quant(x)
+
+
+def npu_mx_dequant(codes: torch.Tensor, scale: torch.Tensor, *, dst_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that :func:`npu_dynamic_mx_quant`'s codes and scales stand for."""
+    return kernels.mx_dequant(codes, scale, dst_type)
+
+
+def npu_add_rms_norm_dynamic_quant(x1: torch.Tensor, x2: torch.Tensor | None, gamma: torch.Tensor, *,
+                                   beta: torch.Tensor | None = None, epsilon: float = 1e-6, dst_type=torch.int8):
+    """Residual addition, RMS norm and quantisation of hidden states [..., H] in one launch: ``x = x1 + x2``,
+    ``y = x / sqrt(mean(x ** 2) + epsilon) * gamma (+ beta)``, both in the dtype of x1, and what
+    :func:`npu_dynamic_quant` (``dst_type=torch.int8``) or :func:`npu_dynamic_mx_quant` (``torch.float4_e2m1fn_x2``) make
+    of ``y``.  Returns ``(q, scale, y, x)``.  ``x2=None``: no addition, ``x`` is x1.  ``gamma`` and ``beta`` in the dtype
+    of x1 or in float32."""
+    if dst_type == torch.int8:
+        kind = kernels.NORM_INT8
+    else:
+        _require_fp4("npu_add_rms_norm_dynamic_quant", dst_type)
+        kind = kernels.NORM_MXFP4
+    return kernels.add_rms_norm_quant(x1, x2, gamma, beta, epsilon, kind)
+
+
+def npu_format_cast_mx(weight: torch.Tensor, scale: torch.Tensor):
+    """MXFP4 weights in checkpoint order, codes [E, N, K / 2] (or [N, K / 2]) and scales [E, N, K / 32], to the storage of the
+    products; call it once, after loading.  N is a multiple of 32, K of 64."""
+    if weight.dim() == 2:
+        w, s = kernels.format_cast_mx(weight.unsqueeze(0), scale.unsqueeze(0))
+        return w.squeeze(0), s.squeeze(0)
+    return kernels.format_cast_mx(weight, scale)
+
+
+def _one_tensor(t, op: str, name: str):
+    if isinstance(t, (list, tuple)):
+        if len(t) != 1:
+            raise NotImplementedError(f"{op}: one {name} tensor for all experts is expected")
+        return t[0]
+    return t
+
+
+def npu_grouped_matmul_swiglu_quant_v2(x, weight, weight_scale, x_scale, group_list, *, smooth_scale=None,
+                                       weight_assist_matrix=None, bias=None, dequant_mode=2, dequant_dtype=torch.float32,
+                                       quant_mode=2, quant_dtype=None, group_list_type=0, tuning_config=None,
+                                       swiglu_limit: float = 0.0, row_map=None):
+    """gate_up product of MXFP4 rows, SwiGLU and MXFP4 quantisation (the call of ``vllm_ascend/device/device_op.py:208-234``
+    with MXFP weights): ``x`` codes [M, K / 2], ``x_scale`` [M, K / 32], ``weight`` [E, 2 I, K / 2] and ``weight_scale`` as
+    :func:`npu_format_cast_mx` returns them.  Returns (codes [rows, I / 2], scales [rows, I / 32]).  ``row_map`` (extension):
+    int32, the row of ``x`` of every row sorted by expert; without it the rows of ``x`` are sorted."""
+    op = "npu_grouped_matmul_swiglu_quant_v2"
+    if smooth_scale is not None or weight_assist_matrix is not None or bias is not None:
+        raise NotImplementedError(f"{op}: smooth_scale / weight_assist_matrix / bias are not supported")
+    if dequant_mode != 2 or quant_mode != 2 or dequant_dtype != torch.float32:
+        raise NotImplementedError(f"{op}: the MX form only (dequant_mode=2, quant_mode=2, dequant_dtype=torch.float32)")
+    _require_fp4(op, quant_dtype)
+    return kernels.gmm_mx_swiglu_quant(x, x_scale, _one_tensor(weight, op, "weight"), _one_tensor(weight_scale, op, "scale"),
+                                       group_list, group_list_type, swiglu_limit, row_map)
+
+
+def _mx_quant_matmul(x1, x2, scale, offset, pertoken_scale, bias, output_dtype):
+    if offset is not None or bias is not None or pertoken_scale is None:
+        raise NotImplementedError("npu_quant_matmul: MXFP4 rows need pertoken_scale and take neither offset nor bias")
+    if output_dtype not in (None, torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"npu_quant_matmul: output_dtype {output_dtype} is not supported")
+    if x2.dim() != 2 or scale.dim() != 2:
+        raise ValueError("npu_quant_matmul: MXFP4 weights are [N, K / 2], their scales [N, columns] (npu_format_cast_mx)")
+    lead = x1.shape[:-1]
+    rows = x1.reshape(-1, x1.shape[-1])
+    out = kernels.gmm_mx(rows, pertoken_scale.reshape(-1, pertoken_scale.shape[-1]), x2.unsqueeze(0), scale.unsqueeze(0),
+                         None, 0, output_dtype or torch.bfloat16)
+    return out.reshape(*lead, x2.shape[0])

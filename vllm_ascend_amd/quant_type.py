@@ -1,5 +1,5 @@
 """Quantisation kinds of the MoE schemes (mirror of ``vllm_ascend/quantization/quant_type.py:26-37``).
-Only NONE, W8A8 and W4A8 have kernels on MI355X; the other members exist so that
+Only NONE, W8A8, W4A8 and W4A4MXFP have kernels on MI355X; the other members exist so that
 callers can name them and get a clear NotImplementedError."""
 from enum import Enum
 
@@ -16,4 +16,4 @@ class QuantType(Enum):
     W4A16MXFP = 8
 
 
-SUPPORTED = (QuantType.W8A8, QuantType.W4A8)
+SUPPORTED = (QuantType.W8A8, QuantType.W4A8, QuantType.W4A4MXFP)
