@@ -16,6 +16,8 @@
 // scales that lie some powers of two apart.  So the order of K, and its split over wavefronts, hardly ever shows.
 #pragma once
 
+#include <type_traits>
+
 #include "mx_common.h"
 
 namespace moe355 {
@@ -47,6 +49,12 @@ __device__ __forceinline__ v16f mfma_mx(v4i a, v4i b, v16f c, int sa, int sb, in
     case 2: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 2, sa, 2, sb);
     default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 3, sa, 3, sb);
     }
+}
+
+// `bytes` of memory for buffer loads: an offset past them reads as zero
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, int bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
 }
 
 // Rows [row0, row1) of expert e, inside [0, rows) whatever the list holds.  Every lane of a wavefront calls it.
@@ -81,16 +89,18 @@ __device__ __forceinline__ float swiglu_f64(float g, float u)
     return (float)(d / (1.0 + exp(-d)) * (double)u);
 }
 
-// 16 values of silu(gate) * up a lane.
+// A block of 32 output channels of a token, of which this lane has 16: silu(gate) * up to MXFP4, codes 16 bytes at `codes`, its
+// scale at `scale`.  Both halves of the wavefront call it together; `store`: whether the lane's token exists.
 //
-// What is quantised is the value of the formula, rounded to binary32.  m_silu and the product are a few units in the last place
-// off it, which shows in the codes only next to a border: the middles between two codes and the powers of two where the scale
-// changes, all of which have a mantissa of two bits and then zeros.  A value within 16 units of such a number (1.5 in 10^5 of
-// them) is computed again in 64 bits, and so is one whose gate is below -80, where m_silu ends.  The codes are therefore those
-// of the formula whatever exp is used, for 2 instructions a value.
-__device__ __forceinline__ void mx_swiglu(v16f& g, const v16f& up, float limit)
+// What is quantised is the value of the formula, rounded to binary32.  The hardware's exp2 and reciprocal make it in 13 issue
+// slots a value (a transcendental instruction takes four; the IEEE sequence of the int8 epilogues takes 30), off by at most
+// 48 units in the last place for gates above -32: |g| 7.5e-8 from the rounded argument of exp2, 4e-7 from the rest.  That shows
+// in the codes only next to a border: the middles between two codes and the powers of two where the scale changes, all of
+// which have a mantissa of two bits and then zeros.  A value within 64 units of such a number (6 in 10^5 of them; infinities
+// and NaN look like one) is computed again in 64 bits, and so is one with a gate below -32, unless it is small enough beside its
+// block to have the code of zero anyway.  The codes are therefore those of the formula, bit for bit.
+__device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int half, bool store, uint8_t* codes, uint8_t* scale)
 {
-    v16f u = up;
     if (limit > 0.0f) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -99,23 +109,35 @@ __device__ __forceinline__ void mx_swiglu(v16f& g, const v16f& up, float limit)
             u[i] = u[i] < -limit ? -limit : u[i];
         }
     }
-    v16f y;
+    constexpr uint32_t kNear = 64;
+    float y[16];
     uint32_t near = 0xffffffffu;
-    float least = 0.0f;
+    float least = 0.0f, m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        y[i] = m_silu(g[i]) * u[i];
-        const uint32_t key = (__float_as_uint(y[i]) << 11) + (16u << 11);
+        const float e = __builtin_amdgcn_exp2f(g[i] * -1.44269504088896341f);
+        y[i] = g[i] * u[i] * __builtin_amdgcn_rcpf(1.0f + e);
+        const uint32_t key = (__float_as_uint(y[i]) << 11) + (kNear << 11);
         near = key < near ? key : near;
-        least = g[i] < least ? g[i] : least;
+        least = __builtin_fminf(least, g[i]);
+        m = __builtin_fmaxf(m, __builtin_fabsf(y[i]));  // passes over NaN, which `near` sees
     }
-    if (near < (32u << 11) || least < -80.0f) {
+    auto block_scale = [&](uint32_t bits) {
+        const v2u both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+        return mx_scale(max_u32(both[0], both[1]));
+    };
+    MxScale s = block_scale(__float_as_uint(m));
+    if (__any(store && (near < (2 * kNear << 11) || least < -32.0f))) {
         uint32_t todo = 0;
+        // over 2^e a value below 0.1 has the code of zero, even if the block's scale turns out to be half as large
+        const float small = 0.1f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const uint32_t key = (__float_as_uint(y[i]) << 11) + (16u << 11);
-            if ((key < (32u << 11) || g[i] < -80.0f) && g[i] != 0.0f && u[i] != 0.0f) todo |= 1u << i;
+            const uint32_t key = (__float_as_uint(y[i]) << 11) + (kNear << 11);
+            const bool number = __builtin_fabsf(y[i]) * s.inverse < small;  // false for NaN
+            if ((key < (2 * kNear << 11) || g[i] < -32.0f) && !(number && s.finite && s.byte > 0)) todo |= 1u << i;
         }
+        if (!store) todo = 0;
         while (todo) {
             const int at = __builtin_ctz(todo);
             todo &= todo - 1;
@@ -126,19 +148,11 @@ __device__ __forceinline__ void mx_swiglu(v16f& g, const v16f& up, float limit)
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[i] = i == at ? v : y[i];
         }
-    }
-    g = y;
-}
-
-// A block of 32 channels of a token (this lane's 16 of them in y) to MXFP4: codes 16 bytes at `codes`, its scale at `scale`.
-// Both halves of the wavefront call it together; `store`: whether the lane's token exists.
-__device__ __forceinline__ void mx_store_block(const v16f& y, int half, bool store, uint8_t* codes, uint8_t* scale)
-{
-    uint32_t m = 0;
+        uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max_u32(m, __float_as_uint(y[i]) & 0x7fffffffu);
-    const v2u both = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-    const MxScale s = mx_scale(max_u32(both[0], both[1]));
+        for (int i = 0; i < 16; ++i) bits = max_u32(bits, __float_as_uint(y[i]) & 0x7fffffffu);
+        s = block_scale(bits);
+    }
     float v[2][8];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = y[i] * s.inverse;
@@ -174,5 +188,10 @@ __device__ __forceinline__ void mx_store_half(const v16f& y, int half, bool stor
         if (store) *(v4u*)(to + 16 * p + 8 * half) = v;
     }
 }
+
+// The product with 128 x 256 tiles (gmm_mx_tiled.hip), and the bytes of its list of tiles.
+bool mx_tiled_takes(const MxArgs& a);  // offsets of 32 bits reach all rows, and there are four scales at least
+int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st);
+size_t mx_tiled_workspace(int64_t rows, int num_experts);
 
 }  // namespace moe355

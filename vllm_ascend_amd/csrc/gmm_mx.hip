@@ -81,8 +81,8 @@ __global__ __launch_bounds__(64 * kWaves) void gmm_mx_stream_kernel(MxArgs a)
                 }
             const bool store = row < row1;
             if constexpr (EPI == MX_SWIGLU) {
-                mx_swiglu(acc0, acc1, a.limit);
-                mx_store_block(acc0, half, store, (uint8_t*)a.out + row * (a.N / 4) + t0 * 16, a.out_scale + row * (a.N / 64) + t0);
+                mx_swiglu_store(acc0, acc1, a.limit, half, store, (uint8_t*)a.out + row * (a.N / 4) + t0 * 16,
+                                a.out_scale + row * (a.N / 64) + t0);
             } else {
                 uint16_t* to = (uint16_t*)a.out + row * a.N;
                 mx_store_half<DT>(acc0, half, store, to + t0 * 32);
@@ -105,12 +105,13 @@ int check(const MxArgs& a, bool swiglu)
     return MOE355_OK;
 }
 
-int run(const MxArgs& a, bool swiglu, int out_dtype, hipStream_t st)
+int run(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)
 {
     if (const int rc = check(a, swiglu)) return rc;
     if (a.rows == 0) return MOE355_OK;
     if (!a.x || !a.x_scale || !a.w || !a.w_scale || (!a.group_list && a.E > 1) || !a.out || (swiglu && !a.out_scale)) return MOE355_E_ARG;
     if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.w_scale, 4) || !aligned(a.out, 16)) return MOE355_E_SHAPE;
+    if (a.rows >= 48 * (int64_t)a.E && mx_tiled_takes(a)) return launch_mx_tiled(a, swiglu, out_dtype, workspace, workspace_bytes, st);
     const dim3 grid((unsigned)((a.N / 32 + 1) / 2), (unsigned)a.E);
     if (swiglu) hipLaunchKernelGGL((gmm_mx_stream_kernel<MX_SWIGLU, MOE355_DT_BF16>), grid, dim3(64 * kWaves), 0, st, a);
     else if (out_dtype == MOE355_DT_BF16)
@@ -140,8 +141,8 @@ extern "C" int moe355_format_cast_mx(const uint8_t* codes, const uint8_t* scale,
 
 extern "C" size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int64_t k, int num_experts)
 {
-    (void)rows, (void)n, (void)k, (void)num_experts;
-    return 256;
+    (void)n, (void)k;
+    return rows > 0 && num_experts > 0 ? mx_tiled_workspace(rows, num_experts) : 256;
 }
 
 extern "C" int moe355_gmm_mx(const uint8_t* x, const uint8_t* x_scale, const int32_t* row_token, int64_t x_rows,
@@ -149,11 +150,10 @@ extern "C" int moe355_gmm_mx(const uint8_t* x, const uint8_t* x_scale, const int
                              int64_t rows, int64_t k, int64_t n, int num_experts, void* out, int out_dtype, void* workspace,
                              size_t workspace_bytes, void* stream)
 {
-    (void)workspace, (void)workspace_bytes;
     if (out_dtype != MOE355_DT_BF16 && out_dtype != MOE355_DT_F16) return MOE355_E_ARG;
     const MxArgs a = {x, x_scale, row_token, w, w_scale, group_list, group_list_type, rows, x_rows, k, n, num_experts, 0.0f,
                       out, nullptr};
-    return run(a, false, out_dtype, (hipStream_t)stream);
+    return run(a, false, out_dtype, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int moe355_gmm_mx_swiglu_quant(const uint8_t* x, const uint8_t* x_scale, const int32_t* row_token, int64_t x_rows,
@@ -162,8 +162,7 @@ extern "C" int moe355_gmm_mx_swiglu_quant(const uint8_t* x, const uint8_t* x_sca
                                           float swiglu_limit, uint8_t* out, uint8_t* out_scale, void* workspace,
                                           size_t workspace_bytes, void* stream)
 {
-    (void)workspace, (void)workspace_bytes;
     const MxArgs a = {x, x_scale, row_token, w, w_scale, group_list, group_list_type, rows, x_rows, k, n, num_experts,
                       swiglu_limit, out, out_scale};
-    return run(a, true, MOE355_DT_BF16, (hipStream_t)stream);
+    return run(a, true, MOE355_DT_BF16, workspace, workspace_bytes, (hipStream_t)stream);
 }

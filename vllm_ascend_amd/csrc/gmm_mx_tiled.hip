@@ -1,0 +1,304 @@
+// Products of MXFP4 rows and weights for many rows an expert.
+//
+// A workgroup of four wavefronts has a tile of 128 tokens x 256 channels (128 gate channels and their 128 up channels for
+// SwiGLU), a wavefront 64 of those channels (a gate block and its up block) with all the tokens: 2 x 4 products of 32 x 32, 128
+// accumulators a lane.  Tokens come through LDS, three windows of 256 K in a ring, by LDS-direct loads two windows ahead;
+// weights go straight from the caches to registers in the order of their storage, one window ahead, since no other wavefront
+// of the workgroup reads them.  A step of 64 K takes 8 matrix instructions of 32 cycles, 2 KiB of weights and 4 KiB of
+// tokens a wavefront: 64 of the 128 bytes a cycle that LDS gives, 48 of the 64 of the L1.  Two workgroups share a compute unit, so
+// that the vector instructions of one's epilogue run beside the other's matrix instructions.
+#include "gmm_mx.h"
+
+namespace moe355 {
+namespace {
+
+constexpr int kTileRows = 128, kTileTiles = 8;  // tokens, blocks of 32 channels
+constexpr int kThreads = 256;
+constexpr int kRing = 3;
+constexpr int kStage = kTileRows * 128;  // tokens' bytes of a window
+constexpr int kLds = kRing * (kStage + kTileRows * 8);
+
+#define MOE355_GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
+#define MOE355_LPTR(p) ((__attribute__((address_space(3))) void*)(p))
+
+// (expert, rows) of the tiles, in the order of the experts
+struct MxMap {
+    int32_t* count;
+    int32_t *expert, *begin, *end;
+};
+inline int64_t most_tiles(int64_t rows, int E) { return rows / kTileRows + (rows < E ? rows : E); }
+inline MxMap map_in(void* p, int64_t most)
+{
+    int32_t* q = (int32_t*)p;
+    return {q, q + 64, q + 64 + most, q + 64 + 2 * most};
+}
+
+// One workgroup; thread t has the experts [t seg, (t + 1) seg).  Rows are cut to those that exist.
+__global__ __launch_bounds__(1024) void mx_map_kernel(const int64_t* __restrict__ list, int gl_type, int E, int64_t rows, MxMap map,
+                                                     int32_t most)
+{
+    __shared__ int64_t sums[16];
+    __shared__ int32_t tiles_of[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = (E + 1023) / 1024;
+    const int e0 = tid * seg, e1 = e0 + seg < E ? e0 + seg : E;
+    int64_t mine = 0, before = 0;
+    if (gl_type == MOE355_GL_COUNT) {
+        for (int e = e0; e < e1; ++e) {
+            const int64_t n = list[e];
+            mine += n < 0 ? 0 : n < rows ? n : rows;
+        }
+        int64_t inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t o = __shfl_up(inc, off, 64);
+            if (lane >= off) inc += o;
+        }
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
+        before = inc - mine;
+        for (int w = 0; w < wave; ++w) before += sums[w];
+    }
+    auto range = [&](int e, int64_t& row, int64_t& r0, int64_t& r1) {
+        if (gl_type == MOE355_GL_COUNT) {
+            const int64_t n = list[e];
+            r0 = row;
+            r1 = r0 + (n < 0 ? 0 : n < rows ? n : rows);
+            row = r1;
+        } else {
+            r0 = e > 0 ? list[e - 1] : 0;
+            r1 = list[e];
+        }
+        r0 = r0 < 0 ? 0 : r0 > rows ? rows : r0;
+        r1 = r1 < r0 ? r0 : r1 > rows ? rows : r1;
+    };
+    int64_t row = before, r0, r1;
+    int32_t tiles = 0;
+    for (int e = e0; e < e1; ++e) {
+        range(e, row, r0, r1);
+        const int32_t n = (int32_t)((r1 - r0 + kTileRows - 1) / kTileRows);
+        tiles = tiles + n < most ? tiles + n : most;  // (a list of sums that goes back and forth may name rows many times)
+    }
+    const int32_t inc = wave_scan_inclusive_i32(tiles);
+    if (lane == 63) tiles_of[wave] = inc < 0 || inc > most ? most : inc;
+    __syncthreads();
+    int64_t at = inc < 0 ? most : inc - tiles, all = 0;
+    for (int w = 0; w < 16; ++w) {
+        if (w < wave) at += tiles_of[w];
+        all += tiles_of[w];
+    }
+    if (tid == 0) map.count[0] = (int32_t)(all < most ? all : most);
+    row = before;
+    for (int e = e0; e < e1; ++e) {
+        range(e, row, r0, r1);
+        for (int64_t r = r0; r < r1 && at < most; r += kTileRows, ++at) {
+            map.expert[at] = e;
+            map.begin[at] = (int32_t)r;
+            map.end[at] = (int32_t)r1;
+        }
+    }
+}
+
+template <int EPI, int DT>
+__global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxMap map)
+{
+    // (not an array of a known size: the compiler would wait for every load on its way to it before each read)
+    extern __shared__ __attribute__((aligned(16))) uint8_t mx_lds[];
+    uint8_t* const tokens = mx_lds;
+    int* const scales = (int*)(mx_lds + kRing * kStage);  // [kRing][rows][2]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int tiles = (int)(a.N / 32), steps = (int)(a.K / 64), windows = (steps + 3) / 4;
+    const int columns = EPI == MX_SWIGLU ? (tiles / 2 + 3) / 4 : (tiles + 7) / 8;
+
+    // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one after
+    // the other, so that the tile's tokens and the expert's weights stay in its L2.
+    const int64_t count = a.group_list ? map.count[0] : (a.rows + kTileRows - 1) / kTileRows;
+    const int64_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= share || item >= items) return;
+    const int tile = (int)(item / columns), column = (int)(item % columns);
+    const int e = a.group_list ? map.expert[tile] : 0;
+    const int64_t row0 = a.group_list ? map.begin[tile] : (int64_t)tile * kTileRows, row1 = a.group_list ? map.end[tile] : a.rows;
+
+    // this wavefront's two blocks of channels (a block past the last one computes the last one again and is not stored)
+    const int b0 = EPI == MX_SWIGLU ? column * 4 + wave : column * 8 + 2 * wave;
+    const int last = EPI == MX_SWIGLU ? tiles / 2 - 1 : tiles - 1;
+    const bool has0 = b0 <= last, has1 = EPI == MX_SWIGLU ? has0 : b0 + 1 <= last;
+    const int t0 = has0 ? b0 : last, t1 = EPI == MX_SWIGLU ? t0 + tiles / 2 : has1 ? b0 + 1 : last;
+    // Buffer loads: their offsets cost no registers, and what lies past the end of an operand is zero without being read.
+    const auto w0 = mx_buffer(a.w + ((int64_t)e * tiles + t0) * steps * 1024, steps * 1024);
+    const auto w1 = mx_buffer(a.w + ((int64_t)e * tiles + t1) * steps * 1024, steps * 1024);
+    const auto ws0 = mx_buffer(a.w_scale + ((int64_t)e * tiles + t0) * windows * 256, windows * 256);
+    const auto ws1 = mx_buffer(a.w_scale + ((int64_t)e * tiles + t1) * windows * 256, windows * 256);
+
+    // Tokens' bytes of a window: row-major, 128 bytes a row, the 16-byte pieces exchanged by row so that the 8 lanes that LDS
+    // serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.
+    auto token_of = [&](int64_t row) -> uint32_t {
+        row = row < row1 ? row : row1 - 1;  // rows behind the last one are not stored
+        if (!a.row_token) return (uint32_t)row;
+        const int64_t t = a.row_token[row];
+        return t >= 0 && t < a.x_rows ? (uint32_t)t : 0;
+    };
+    const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
+    uint32_t from[4];                               // (the rows take less than 4 GiB)
+    const int piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + piece * 16;
+    // scales: thread t has row t / 2, half t % 2
+    const uint32_t scale_from = token_of(row0 + (threadIdx.x >> 1)) * (uint32_t)(a.K / 32);
+
+    auto fetch_tokens = [&](int w, int slot) {
+        // a shorter last window has 32 bytes a step of a row; the pieces behind them are the first one again (not used)
+        const uint32_t back = w < full || piece < 2 * tail ? 0 : piece * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_global_load_lds(MOE355_GPTR(a.x + w * 128 + (from[i] - back)),
+                                             MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16, 0, 0);
+    };
+    const uint32_t scale_end = (uint32_t)(a.x_rows * (a.K / 32)) - 4;  // (the rows have at least four scales)
+    auto fetch_scale = [&](int w) {
+        // the scales of a shorter window are the low bytes of the four from there on, or of what the last four hold of them
+        const uint32_t want = scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail);
+        const uint32_t at = want < scale_end ? want : scale_end;
+        int v;
+        __builtin_memcpy(&v, a.x_scale + at, 4);
+        return (int)((uint32_t)v >> (8 * (want - at)));
+    };
+    struct Weights {
+        v4i a[2][4];
+        int s[2];
+    };
+    auto fetch_weights = [&](int w, Weights& to) {
+        const int at = w * 4096 + lane * 16, scale_at = w * 256 + lane * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            to.a[0][j] = __builtin_amdgcn_raw_buffer_load_b128(w0, at + j * 1024, 0, 0);
+            to.a[1][j] = __builtin_amdgcn_raw_buffer_load_b128(w1, at + j * 1024, 0, 0);
+        }
+        to.s[0] = __builtin_amdgcn_raw_buffer_load_b32(ws0, scale_at, 0, 0);
+        to.s[1] = __builtin_amdgcn_raw_buffer_load_b32(ws1, scale_at, 0, 0);
+    };
+
+    v16f acc[2][4] = {};
+    const int row_in = lane & 31;
+    auto compute = [&](int slot, const Weights& w, int nb, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        int sb[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sb[t] = scales[slot * (2 * kTileRows) + (t * 32 + row_in) * 2 + half];
+        const uint8_t* base = tokens + slot * kStage + row_in * 128;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (WHOLE || j < nb) {
+                const int at = ((half * nb + j) ^ (row_in & 7)) * 16;
+                v4i b[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) b[t] = *(const v4i*)(base + t * 32 * 128 + at);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    acc[0][t] = mfma_mx(w.a[0][j], b[t], acc[0][t], w.s[0], sb[t], j);
+                    acc[1][t] = mfma_mx(w.a[1][j], b[t], acc[1][t], w.s[1], sb[t], j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    Weights held[2];
+    const int own = threadIdx.x, end = windows - 1;
+    auto cut = [&](int w) { return w < end ? w : end; };
+    // prologue: windows 0 and 1 on their way
+    fetch_tokens(0, 0);
+    scales[own] = fetch_scale(0);
+    int scale_next = fetch_scale(cut(1));
+    fetch_tokens(cut(1), 1);
+    fetch_weights(0, held[0]);
+    // Window w: its tokens have been asked for two windows ago, its weights one.  Behind the barrier everybody has read window
+    // w - 1, whose place in the ring window w + 2 takes.
+    int slot = 0;
+    auto window = [&](int w, Weights& now, Weights& next, auto whole) {
+        const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
+        scales[slot1 * (2 * kTileRows) + own] = scale_next;
+        // the 4 loads of the next window's tokens and the 10 of this one's weights may still be on their way
+        asm volatile("s_waitcnt vmcnt(14) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        scale_next = fetch_scale(cut(w + 2));
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_weights(w + 1, next);
+        fetch_tokens(cut(w + 2), slot2);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(slot, now, decltype(whole)::value || w < full ? 4 : tail, whole);
+        __builtin_amdgcn_sched_barrier(0);
+        slot = slot1;
+    };
+    constexpr std::true_type whole{};
+    constexpr std::false_type part{};
+    int w = 0;
+    for (; w + 1 < full; w += 2) {
+        window(w, held[0], held[1], whole);
+        window(w + 1, held[1], held[0], whole);
+    }
+    for (; w < windows; ++w) {  // at most two more, of which the last one may be short
+        window(w, held[0], held[1], part);
+        held[0] = held[1];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end still write LDS
+
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int64_t row = row0 + t * 32 + row_in;
+        const bool store = row < row1 && has0;
+        if (a.row_token) {  // a row that is not there counts as zeros
+            const int64_t token = row < row1 ? a.row_token[row] : 0;
+            const bool there = token >= 0 && token < a.x_rows;
+            if (__any(!there)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    acc[0][t][i] = there ? acc[0][t][i] : 0.0f;
+                    acc[1][t][i] = there ? acc[1][t][i] : 0.0f;
+                }
+            }
+        }
+        if constexpr (EPI == MX_SWIGLU) {
+            mx_swiglu_store(acc[0][t], acc[1][t], a.limit, half, store, (uint8_t*)a.out + row * (a.N / 4) + t0 * 16,
+                            a.out_scale + row * (a.N / 64) + t0);
+        } else {
+            uint16_t* to = (uint16_t*)a.out + row * a.N;
+            mx_store_half<DT>(acc[0][t], half, store, to + t0 * 32);
+            mx_store_half<DT>(acc[1][t], half, row < row1 && has1, to + t1 * 32);
+        }
+    }
+}
+
+}  // namespace
+
+size_t mx_tiled_workspace(int64_t rows, int num_experts)
+{
+    return (size_t)((64 + 3 * most_tiles(rows, num_experts)) * 4 + 255) / 256 * 256;
+}
+
+bool mx_tiled_takes(const MxArgs& a)
+{
+    return a.x_rows * (a.K / 2) < (int64_t)1 << 32 && a.x_rows * (a.K / 32) >= 4;
+}
+
+int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)
+{
+    const int64_t most = a.group_list ? most_tiles(a.rows, a.E) : (a.rows + kTileRows - 1) / kTileRows;
+    const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, groups = (most * columns + 7) / 8 * 8;
+    if (groups > 0x7fffffff) return MOE355_E_SHAPE;
+    MxMap map = {};
+    if (a.group_list) {
+        if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < mx_tiled_workspace(a.rows, a.E))
+            return MOE355_E_WORKSPACE;
+        map = map_in(workspace, most);
+        hipLaunchKernelGGL(mx_map_kernel, dim3(1), dim3(1024), 0, st, a.group_list, a.gl_type, a.E, a.rows, map, (int32_t)most);
+    }
+    const dim3 grid((unsigned)groups);
+    if (swiglu) hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_SWIGLU, MOE355_DT_BF16>), grid, dim3(kThreads), kLds, st, a, map);
+    else if (out_dtype == MOE355_DT_BF16)
+        hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_HALF, MOE355_DT_BF16>), grid, dim3(kThreads), kLds, st, a, map);
+    else hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_HALF, MOE355_DT_F16>), grid, dim3(kThreads), kLds, st, a, map);
+    return launch_status();
+}
+
+}  // namespace moe355
