@@ -611,9 +611,10 @@ int moe355_format_cast_mx(const uint8_t *codes, const uint8_t *scale, int64_t nu
  *                                out_scale [rows, n / 64] of its MXFP4 form
  * Stand in for torch_npu.npu_grouped_matmul and npu_grouped_matmul_swiglu_quant_v2 with E8M0 scales (the MXFP4 branch of
  * vllm_ascend/device/device_op.py:208-291).
- * Row r of the sorted rows is row row_token[r] of x (NULL: row r, x_rows = rows); one outside [0, x_rows) counts as zeros.
+ * Row r of the sorted rows is row row_token[r] of x (NULL: row r, x_rows = rows); one outside [0, x_rows) counts as zeros (x_rows > 0).
  * The group list (int64, meaning as above; NULL: one expert, all rows) is cut to [0, rows); rows behind the last group are left as they were.
- * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; x, w, out 16-byte aligned. */
+ * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; x, w, out 16-byte aligned; x_rows * k / 2 below 4 GiB less
+ * 1 MiB; the memory at x_scale has four bytes even where one row of k = 64 has two. */
 size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int64_t k, int num_experts);
 int moe355_gmm_mx(const uint8_t *x, const uint8_t *x_scale, const int32_t *row_token, int64_t x_rows, const uint8_t *w,
                   const uint8_t *w_scale, const int64_t *group_list, int group_list_type, int64_t rows, int64_t k, int64_t n,

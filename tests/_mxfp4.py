@@ -65,12 +65,11 @@ def swiglu(acc, limit=0.0):
 
 
 def random_mx(rng, shape, spread=2, heavy=False):
-    """Codes 0..15 and scales of random rows [..., K] as quantisation leaves them, `spread` powers of two apart."""
-    v = rng.standard_normal(shape)
+    """Codes 0..15 and scales of random rows [..., K], blocks `spread` powers of two apart; heavy: large codes are rare."""
+    code = rng.integers(0, 16, shape, dtype=np.uint8)
     if heavy:
-        v = v * rng.standard_normal(shape)
-    v = v * np.exp2(rng.integers(0, spread + 1, (*shape[:-1], shape[-1] // 32))).repeat(32, -1)
-    return quantise(v)
+        code &= rng.integers(0, 16, shape, dtype=np.uint8) | 8
+    return code, (127 - 2 + rng.integers(0, spread + 1, (*shape[:-1], shape[-1] // 32))).astype(np.uint8)
 
 
 def rounded(v, dtype):

@@ -78,7 +78,7 @@ def test_products_refuse(lib):
                     dict(rows=-1), dict(x_rows=-1), dict(k=0), dict(n=0), dict(E=0)):
             assert call(swiglu, **bad) == -1, bad
         for bad in (dict(k=96), dict(n=48), dict(x=P + 8), dict(w=P + 8), dict(ws=P + 2), dict(out=P + 8), dict(rows=1 << 31),
-                    dict(x_rows=1 << 31), dict(E=1 << 20), dict(k=1 << 21), dict(n=1 << 21)):
+                    dict(x_rows=1 << 31), dict(E=1 << 20), dict(k=1 << 21), dict(n=1 << 21), dict(x_rows=1 << 26)):
             assert call(swiglu, **bad) == -2, bad
     assert call(True, n=96) == -2 and call(True, out_scale=None) == -1 and call(False, dt=0) == -1
     f = lib.moe355_format_cast_mx

@@ -52,9 +52,22 @@ __device__ __forceinline__ v16f mfma_mx(v4i a, v4i b, v16f c, int sa, int sb, in
 }
 
 // `bytes` of memory for buffer loads: an offset past them reads as zero
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, int bytes)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+}
+
+// Scales of a row from offset `want` on, the first one in the low byte, as many of four as there are: at the end of the memory the
+// last four bytes, shifted.
+__device__ __forceinline__ uint32_t mx_scale_bytes(const MxArgs& a)
+{
+    const int64_t n = a.x_rows * (a.K / 32);
+    return (uint32_t)(n < 4 ? 4 : n);  // (the caller's memory has four)
+}
+__device__ __forceinline__ int mx_row_scales(__amdgpu_buffer_rsrc_t scales, uint32_t want, uint32_t end)
+{
+    const uint32_t at = want < end ? want : end;
+    return (int)((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(scales, at, 0, 0) >> (8 * (want - at)));
 }
 
 // Rows [row0, row1) of expert e, inside [0, rows) whatever the list holds.  Every lane of a wavefront calls it.
@@ -190,7 +203,6 @@ __device__ __forceinline__ void mx_store_half(const v16f& y, int half, bool stor
 }
 
 // The product with 128 x 256 tiles (gmm_mx_tiled.hip), and the bytes of its list of tiles.
-bool mx_tiled_takes(const MxArgs& a);  // offsets of 32 bits reach all rows, and there are four scales at least
 int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st);
 size_t mx_tiled_workspace(int64_t rows, int num_experts);
 

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         return t >= 0 && t < a.x_rows ? (uint32_t)t : 0;
     };
     const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
-    uint32_t from[4];                               // (the rows take less than 4 GiB)
+    uint32_t from[4];
     const int piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
     for (int i = 0; i < 4; ++i) from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + piece * 16;
@@ -153,14 +153,10 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
             __builtin_amdgcn_global_load_lds(MOE355_GPTR(a.x + w * 128 + (from[i] - back)),
                                              MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16, 0, 0);
     };
-    const uint32_t scale_end = (uint32_t)(a.x_rows * (a.K / 32)) - 4;  // (the rows have at least four scales)
+    const uint32_t scale_end = mx_scale_bytes(a) - 4;
+    const auto x_scales = mx_buffer(a.x_scale, scale_end + 4);
     auto fetch_scale = [&](int w) {
-        // the scales of a shorter window are the low bytes of the four from there on, or of what the last four hold of them
-        const uint32_t want = scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail);
-        const uint32_t at = want < scale_end ? want : scale_end;
-        int v;
-        __builtin_memcpy(&v, a.x_scale + at, 4);
-        return (int)((uint32_t)v >> (8 * (want - at)));
+        return mx_row_scales(x_scales, scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail), scale_end);
     };
     struct Weights {
         v4i a[2][4];
@@ -274,11 +270,6 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
 size_t mx_tiled_workspace(int64_t rows, int num_experts)
 {
     return (size_t)((64 + 3 * most_tiles(rows, num_experts)) * 4 + 255) / 256 * 256;
-}
-
-bool mx_tiled_takes(const MxArgs& a)
-{
-    return a.x_rows * (a.K / 2) < (int64_t)1 << 32 && a.x_rows * (a.K / 32) >= 4;
 }
 
 int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)

@@ -42,11 +42,12 @@ class AscendRoutedExperts(torch.nn.Module):
         # ... and, for at most 1024 (token, slot) pairs, without sorting them: every intermediate row belongs to a
         # pair, the GEMMs' workgroups collect the pairs of their expert themselves (W8A8 scheme)
         self.use_pair_order = True
-        specs = dict(quant_method.get_weight(moe_config.num_experts, moe_config.intermediate_size_per_partition,
-                                             moe_config.hidden_dim, params_dtype))
-        specs.update(quant_method.get_dynamic_quant_param(moe_config.num_experts,
-                                                          moe_config.intermediate_size_per_partition,
-                                                          moe_config.hidden_dim, params_dtype))
+        with torch.device(device):  # made where they stay: gigabytes need not cross the bus
+            specs = dict(quant_method.get_weight(moe_config.num_experts, moe_config.intermediate_size_per_partition,
+                                                 moe_config.hidden_dim, params_dtype))
+            specs.update(quant_method.get_dynamic_quant_param(moe_config.num_experts,
+                                                              moe_config.intermediate_size_per_partition,
+                                                              moe_config.hidden_dim, params_dtype))
         for name, t in specs.items():
             self.register_parameter(name, torch.nn.Parameter(t.to(device), requires_grad=False))
         self.moe_comm_method = setup_moe_comm_method(moe_config)

@@ -1005,7 +1005,11 @@ def _mx_operands(op, x, x_scale, weight, weight_scale, group_list, row_map, n_mu
         if row_map.dtype != torch.int32 or row_map.dim() != 1:
             raise TypeError(f"{op}: row_map must be a vector of int32, got {tuple(row_map.shape)} {row_map.dtype}")
         rows, row_map = row_map.numel(), _dev(row_map, "row_map")
+        if rows and not x.shape[0]:
+            raise ValueError(f"{op}: row_map names {rows} rows of an empty x")
     x, x_scale = _flat(x, "x"), _dev(x_scale, "x_scale")
+    if x_scale.numel() < 4:
+        x_scale = torch.nn.functional.pad(x_scale.reshape(-1), (0, 4 - x_scale.numel()))  # the kernels read four at a time
     weight, weight_scale = _flat(weight, "weight"), _flat(weight_scale, "weight_scale")
     group_list = None if group_list is None else _gl(group_list)
     _on(x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, row_map=row_map)
