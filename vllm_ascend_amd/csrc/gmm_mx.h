@@ -57,18 +57,23 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint3
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
 }
 
-// Scales of a row from offset `want` on, the first one in the low byte, as many of four as there are: at the end of the memory the
-// last four bytes, shifted.
 __device__ __forceinline__ uint32_t mx_scale_bytes(const MxArgs& a)
 {
     const int64_t n = a.x_rows * (a.K / 32);
     return (uint32_t)(n < 4 ? 4 : n);  // (the caller's memory has four)
 }
-__device__ __forceinline__ int mx_row_scales(__amdgpu_buffer_rsrc_t scales, uint32_t want, uint32_t end)
-{
-    const uint32_t at = want < end ? want : end;
-    return (int)((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(scales, at, 0, 0) >> (8 * (want - at)));
-}
+// Scales of a row from an offset on, the first one in the low byte, as many of four as there are: at the end of the memory the last
+// four bytes, shifted where they are used (a shift behind the load would wait for it).
+struct MxRowScales {
+    uint32_t raw, shift;
+    __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t scales, uint32_t want, uint32_t end)
+    {
+        const uint32_t at = want < end ? want : end;
+        raw = __builtin_amdgcn_raw_buffer_load_b32(scales, at, 0, 0);
+        shift = 8 * (want - at);
+    }
+    __device__ __forceinline__ int get() const { return (int)(raw >> shift); }
+};
 
 // Rows [row0, row1) of expert e, inside [0, rows) whatever the list holds.  Every lane of a wavefront calls it.
 __device__ __forceinline__ void mx_expert_rows(const MxArgs& a, int e, int lane, int64_t& row0, int64_t& row1)

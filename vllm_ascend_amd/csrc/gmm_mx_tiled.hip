@@ -7,7 +7,7 @@
 // of the workgroup reads them.  A step of 64 K takes 8 matrix instructions of 32 cycles, 2 KiB of weights and 4 KiB of
 // tokens a wavefront: 64 of the 128 bytes a cycle that LDS gives, 48 of the 64 of the L1.  Two workgroups share a compute unit, so
 // that the vector instructions of one's epilogue run beside the other's matrix instructions.
-#include "gmm_mx.h"
+#include "gmm_mx_stream.h"
 
 namespace moe355 {
 namespace {
@@ -123,6 +123,14 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const int last = EPI == MX_SWIGLU ? tiles / 2 - 1 : tiles - 1;
     const bool has0 = b0 <= last, has1 = EPI == MX_SWIGLU ? has0 : b0 + 1 <= last;
     const int t0 = has0 ? b0 : last, t1 = EPI == MX_SWIGLU ? t0 + tiles / 2 : has1 ? b0 + 1 : last;
+    // A short tile: each wavefront by itself, without LDS
+    if (row1 - row0 <= 64) {
+        MxStream<EPI, DT> s = {a, nullptr, lane, half, 0, 1, 0, 0, 0, windows, t0, t1, has0, has1};
+        s.operands(e);
+        if (row1 - row0 <= 32) return s.template rows<1, true>(row0, row1);
+        return s.template rows<2, true>(row0, row1);
+    }
+
     // Buffer loads: their offsets cost no registers, and what lies past the end of an operand is zero without being read.
     const auto w0 = mx_buffer(a.w + ((int64_t)e * tiles + t0) * steps * 1024, steps * 1024);
     const auto w1 = mx_buffer(a.w + ((int64_t)e * tiles + t1) * steps * 1024, steps * 1024);
@@ -156,73 +164,84 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const uint32_t scale_end = mx_scale_bytes(a) - 4;
     const auto x_scales = mx_buffer(a.x_scale, scale_end + 4);
     auto fetch_scale = [&](int w) {
-        return mx_row_scales(x_scales, scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail), scale_end);
+        MxRowScales s;
+        s.fetch(x_scales, scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail), scale_end);
+        return s;
     };
     struct Weights {
         v4i a[2][4];
         int s[2];
     };
+    auto fetch_step = [&](int w, int j, Weights& to) {
+        const int at = w * 4096 + lane * 16;
+        to.a[0][j] = __builtin_amdgcn_raw_buffer_load_b128(w0, at + j * 1024, 0, 0);
+        to.a[1][j] = __builtin_amdgcn_raw_buffer_load_b128(w1, at + j * 1024, 0, 0);
+    };
+    auto fetch_weight_scales = [&](int w, Weights& to) {
+        const int at = w * 256 + lane * 4;
+        to.s[0] = __builtin_amdgcn_raw_buffer_load_b32(ws0, at, 0, 0);
+        to.s[1] = __builtin_amdgcn_raw_buffer_load_b32(ws1, at, 0, 0);
+    };
     auto fetch_weights = [&](int w, Weights& to) {
-        const int at = w * 4096 + lane * 16, scale_at = w * 256 + lane * 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            to.a[0][j] = __builtin_amdgcn_raw_buffer_load_b128(w0, at + j * 1024, 0, 0);
-            to.a[1][j] = __builtin_amdgcn_raw_buffer_load_b128(w1, at + j * 1024, 0, 0);
-        }
-        to.s[0] = __builtin_amdgcn_raw_buffer_load_b32(ws0, scale_at, 0, 0);
-        to.s[1] = __builtin_amdgcn_raw_buffer_load_b32(ws1, scale_at, 0, 0);
+        for (int j = 0; j < 4; ++j) fetch_step(w, j, to);
+        fetch_weight_scales(w, to);
     };
 
     v16f acc[2][4] = {};
     const int row_in = lane & 31;
-    auto compute = [&](int slot, const Weights& w, int nb, auto whole) {
+    auto compute = [&](int slot, Weights& w, int nb, int refill, auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
         int sb[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) sb[t] = scales[slot * (2 * kTileRows) + (t * 32 + row_in) * 2 + half];
         const uint8_t* base = tokens + slot * kStage + row_in * 128;
+        v4i b[4];
+        auto read = [&](int j, int t) { b[t] = *(const v4i*)(base + t * 32 * 128 + ((half * nb + j) ^ (row_in & 7)) * 16); };
+#pragma unroll
+        for (int t = 0; t < 4; ++t) read(0, t);
+        // the next step's tokens into the registers that this step's products have just used, six products ahead
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (WHOLE || j < nb) {
-                const int at = ((half * nb + j) ^ (row_in & 7)) * 16;
-                v4i b[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) b[t] = *(const v4i*)(base + t * 32 * 128 + at);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     acc[0][t] = mfma_mx(w.a[0][j], b[t], acc[0][t], w.s[0], sb[t], j);
                     acc[1][t] = mfma_mx(w.a[1][j], b[t], acc[1][t], w.s[1], sb[t], j);
+                    if (WHOLE ? j < 3 : j + 1 < nb) read(j + 1, t);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (WHOLE) fetch_step(refill, j, w);
         }
+        if constexpr (WHOLE) fetch_weight_scales(refill, w);
     };
 
     Weights held[2];
     const int own = threadIdx.x, end = windows - 1;
     auto cut = [&](int w) { return w < end ? w : end; };
     // prologue: windows 0 and 1 on their way
-    fetch_tokens(0, 0);
-    scales[own] = fetch_scale(0);
-    int scale_next = fetch_scale(cut(1));
-    fetch_tokens(cut(1), 1);
     fetch_weights(0, held[0]);
-    // Window w: its tokens have been asked for two windows ago, its weights one.  Behind the barrier everybody has read window
-    // w - 1, whose place in the ring window w + 2 takes.
+    fetch_weights(1, held[1]);
+    fetch_tokens(0, 0);
+    scales[own] = fetch_scale(0).get();
+    MxRowScales scale_next = fetch_scale(cut(1));
+    fetch_tokens(cut(1), 1);
+    // Window w: its tokens and weights have been asked for two windows ago, a step's weights when the step that had their
+    // registers was done.  Behind the barrier everybody has read window w - 1, whose place in the ring window w + 2 takes.
     int slot = 0;
-    auto window = [&](int w, Weights& now, Weights& next, auto whole) {
+    auto window = [&](int w, Weights& now, auto whole) {
         const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
-        scales[slot1 * (2 * kTileRows) + own] = scale_next;
-        // the 4 loads of the next window's tokens and the 10 of this one's weights may still be on their way
+        scales[slot1 * (2 * kTileRows) + own] = scale_next.get();
+        // behind this window's tokens: the next window's 4 loads of tokens and 10 of weights, at least
         asm volatile("s_waitcnt vmcnt(14) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         scale_next = fetch_scale(cut(w + 2));
         __builtin_amdgcn_sched_barrier(0);
-        fetch_weights(w + 1, next);
         fetch_tokens(cut(w + 2), slot2);
         __builtin_amdgcn_sched_barrier(0);
-        compute(slot, now, decltype(whole)::value || w < full ? 4 : tail, whole);
+        compute(slot, now, decltype(whole)::value || w < full ? 4 : tail, w + 2, whole);
         __builtin_amdgcn_sched_barrier(0);
         slot = slot1;
     };
@@ -230,11 +249,11 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     constexpr std::false_type part{};
     int w = 0;
     for (; w + 1 < full; w += 2) {
-        window(w, held[0], held[1], whole);
-        window(w + 1, held[1], held[0], whole);
+        window(w, held[0], whole);
+        window(w + 1, held[1], whole);
     }
     for (; w < windows; ++w) {  // at most two more, of which the last one may be short
-        window(w, held[0], held[1], part);
+        window(w, held[0], part);
         held[0] = held[1];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end still write LDS
