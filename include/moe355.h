@@ -593,7 +593,7 @@ int moe355_mx_dequant(const uint8_t *codes, const uint8_t *scale, int64_t rows, 
  *   (MOE355_NORM_MXFP4) make of y; MOE355_NORM_PLAIN: y alone.
  * x1, x2, x, y [rows, cols] of x_dtype (bf16 / fp16); gamma, beta [cols] of weight_dtype (x_dtype or fp32), beta may be
  * NULL.  x and y may be NULL (not wanted; MOE355_NORM_PLAIN needs y); x may be the same buffer as x1 or x2.
- * cols % 8 == 0 (MXFP4: 32) and at most 2^20; rows 16-byte aligned. */
+ * cols % 8 == 0 (MXFP4: 32) and at most 2^20; rows and weights 16-byte aligned. */
 enum { MOE355_NORM_PLAIN = 0, MOE355_NORM_INT8 = 1, MOE355_NORM_MXFP4 = 2 };
 int moe355_add_rms_norm_quant(const void *x1, const void *x2, const void *gamma, const void *beta, int x_dtype,
                               int weight_dtype, int64_t rows, int64_t cols, double epsilon, int kind, void *x, void *y,
@@ -615,7 +615,8 @@ int moe355_format_cast_mx(const uint8_t *codes, const uint8_t *scale, int64_t nu
  * The group list (int64, meaning as above; NULL: one expert, all rows) is cut to [0, rows); rows behind the last group are left as they were.
  * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; x, w, out 16-byte aligned; x_rows * k / 2 below 4 GiB less
  * 1 MiB; the memory at x_scale has four bytes even where one row of k = 64 has two. */
-size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int64_t k, int num_experts);
+/* may be 0: no workspace is read then */
+size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int num_experts, int swiglu);
 int moe355_gmm_mx(const uint8_t *x, const uint8_t *x_scale, const int32_t *row_token, int64_t x_rows, const uint8_t *w,
                   const uint8_t *w_scale, const int64_t *group_list, int group_list_type, int64_t rows, int64_t k, int64_t n,
                   int num_experts, void *out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
@@ -623,6 +624,19 @@ int moe355_gmm_mx_swiglu_quant(const uint8_t *x, const uint8_t *x_scale, const i
                                const uint8_t *w, const uint8_t *w_scale, const int64_t *group_list, int group_list_type,
                                int64_t rows, int64_t k, int64_t n, int num_experts, float swiglu_limit, uint8_t *out,
                                uint8_t *out_scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* All MXFP4 experts of a layer on a batch whose routing is known: moe355_dynamic_mx_quant (x_scale NULL: x [T, hidden] of dtype;
+ * otherwise x [T, hidden / 2] and x_scale [T, hidden / 32] are the quantised rows), moe355_route_map, moe355_gmm_mx_swiglu_quant,
+ * moe355_gmm_mx and moe355_token_unpermute in one call, the same bits.  topk_ids [T, k], topk_weights [T, k] of dtype; residual
+ * [T, hidden] of dtype or NULL; expert_tokens [E] receives the counts; out [T, hidden] of dtype (bf16 / fp16).  hidden and
+ * intermediate are multiples of 64, E at most 2048, k at most 64. */
+size_t moe355_mx_experts_workspace(int64_t num_tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts,
+                                   int quantised);
+int moe355_mx_experts(const void *x, const uint8_t *x_scale, int dtype, int64_t num_tokens, int64_t hidden,
+                      const int32_t *topk_ids, const void *topk_weights, int top_k, const uint8_t *w13,
+                      const uint8_t *w13_scale, const uint8_t *w2, const uint8_t *w2_scale, int64_t intermediate,
+                      int num_experts, float swiglu_limit, const void *residual, int64_t *expert_tokens, void *out,
+                      void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -258,8 +258,8 @@ def test_rows_that_no_group_has_stay_as_they_were(K, rows):
     used = int(counts.sum())
     w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
     x, x_scale, lib = dev(ref.pack(xc)), dev(xs), _lib.load()
-    n = lib.moe355_gmm_mx_workspace(rows, N, Kd, E)
-    space = torch.empty(n, dtype=torch.uint8, device=DEV)
+    n = max(lib.moe355_gmm_mx_workspace(rows, N, E, swiglu) for swiglu in (0, 1))
+    space = torch.empty(max(n, 1), dtype=torch.uint8, device=DEV)
     stream = torch.cuda.current_stream().cuda_stream
     want = ref.rounded(ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)[:used], torch.bfloat16)
     for list_type, gl in ((1, counts), (0, counts.cumsum())):

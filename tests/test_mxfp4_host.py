@@ -66,7 +66,7 @@ def test_norm_refuses(lib):
 
 def test_products_refuse(lib):
     def call(swiglu, x=P, xs=P, rt=None, x_rows=4, w=P, ws=P, gl=P, glt=1, rows=4, k=128, n=64, E=2, out=P, out_scale=P, dt=1):
-        space = lib.moe355_gmm_mx_workspace(max(rows, 0), max(n, 0), max(k, 0), max(E, 0))
+        space = lib.moe355_gmm_mx_workspace(rows, n, E, int(swiglu))
         if swiglu:
             return lib.moe355_gmm_mx_swiglu_quant(x, xs, rt, x_rows, w, ws, gl, glt, rows, k, n, E, 0.0, out, out_scale, P, space,
                                                   None)

@@ -138,12 +138,16 @@ PROTOTYPES = {
     "moe355_add_rms_norm_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_double,
                                           c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "moe355_format_cast_mx": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
-    "moe355_gmm_mx_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "moe355_gmm_mx_workspace": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "moe355_gmm_mx": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,
                               c_int64, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "moe355_gmm_mx_swiglu_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64,
                                            c_int64, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
                                            c_void_p]),
+    "moe355_mx_experts_workspace": (c_size_t, [c_int64, c_int, c_int64, c_int64, c_int, c_int]),
+    "moe355_mx_experts": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                  c_void_p]),
 }
 
 _lib = None

@@ -145,15 +145,18 @@ __device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int
         return mx_scale(max_u32(both[0], both[1]));
     };
     MxScale s = block_scale(__float_as_uint(m));
-    if (__any(store && (near < (2 * kNear << 11) || least < -32.0f))) {
+    // (a block of all but nothing, whose products may have lost bits below the normal numbers, too)
+    const bool tiny = s.byte < 32 && m > 0.0f;
+    if (__any(store && (near < (2 * kNear << 11) || least < -32.0f || tiny))) {
         uint32_t todo = 0;
         // over 2^e a value below 0.1 has the code of zero, even if the block's scale turns out to be half as large
         const float small = 0.1f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t key = (__float_as_uint(y[i]) << 11) + (kNear << 11);
-            const bool number = __builtin_fabsf(y[i]) * s.inverse < small;  // false for NaN
-            if ((key < (2 * kNear << 11) || g[i] < -32.0f) && !(number && s.finite && s.byte > 0)) todo |= 1u << i;
+            // (false for NaN; below -80 the exponential ends)
+            const bool nothing = s.finite && !tiny && g[i] >= -80.0f && __builtin_fabsf(y[i]) * s.inverse < small;
+            if ((key < (2 * kNear << 11) || g[i] < -32.0f || tiny) && g[i] != 0.0f && u[i] != 0.0f && !nothing) todo |= 1u << i;
         }
         if (!store) todo = 0;
         while (todo) {
@@ -207,8 +210,24 @@ __device__ __forceinline__ void mx_store_half(const v16f& y, int half, bool stor
     }
 }
 
-// The product with 128 x 256 tiles (gmm_mx_tiled.hip), and the bytes of its list of tiles.
-int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st);
-size_t mx_tiled_workspace(int64_t rows, int num_experts);
+// (expert, rows) of the 128-row tiles, in the order of the experts
+struct MxMap {
+    int32_t* count;
+    int32_t *expert, *begin, *end;
+};
+constexpr int kMxTileRows = 128;
+inline int64_t mx_most_tiles(int64_t rows, int E) { return rows / kMxTileRows + (rows < E ? rows : E); }
+size_t mx_map_bytes(int64_t rows, int num_experts);
+MxMap mx_map_in(void* workspace, int64_t rows, int num_experts);  // 256-byte aligned, mx_map_bytes long
+
+// How a product of this shape runs: every expert's weights streamed by its own workgroups, or tiles, found by each workgroup from
+// the group list or in a list that a launch in front makes (mx_build_map, or the routing launch).
+enum MxForm { MX_STREAM, MX_TILES, MX_LISTED };
+MxForm mx_form(int64_t rows, int64_t n, int num_experts, bool swiglu, bool grouped);
+void mx_build_map(const MxArgs& a, const MxMap& map, hipStream_t st);
+int mx_check(const MxArgs& a, bool swiglu);
+// map: of MX_LISTED.  The arguments have been checked.
+int mx_launch(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, const MxMap& map, hipStream_t st);
+int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, const MxMap& map, hipStream_t st);
 
 }  // namespace moe355

@@ -1,6 +1,5 @@
 // Products of MXFP4 rows with their experts' MXFP4 weights: to 16 bits, or through SwiGLU back to MXFP4.
 #include "gmm_mx_stream.h"
-#include <stdlib.h>
 
 namespace moe355 {
 namespace {
@@ -22,8 +21,8 @@ __global__ __launch_bounds__(256) void mx_format_kernel(const uint8_t* __restric
         for (int64_t j = nb; j < 4; ++j) to_scale[(tile * windows + window) * 256 + lane * 4 + j] = 0;
 }
 
-// Few rows an expert: a workgroup has 64 channels of an expert and all its rows, 32 at a time; its wavefronts have a part of K each
-// and add their sums through LDS.  Three workgroups' wavefronts a SIMD (168 registers), which is why the form of 64 rows is not
+// Few rows an expert: a workgroup has 64 channels of an expert and its rows, 32 at a time (every gridDim.z-th 32); its wavefronts
+// have a part of K each and add their sums through LDS.  Three workgroups' wavefronts a SIMD (168 registers), which is why the form of 64 rows is not
 // here.
 template <int EPI, int DT>
 __global__ __launch_bounds__(512, 3) void gmm_mx_stream_kernel(MxArgs a)
@@ -37,7 +36,7 @@ __global__ __launch_bounds__(512, 3) void gmm_mx_stream_kernel(MxArgs a)
     }
     int64_t row0, row1;
     mx_expert_rows(a, e, lane, row0, row1);
-    if (row0 >= row1) return;
+    if (row0 + 32 * (int64_t)blockIdx.z >= row1) return;
     const int tiles = (int)(a.N / 32), windows = (int)((a.K + 255) / 256);
     MxStream<EPI, DT> s = {a, mx_parts, lane, lane >> 5};
     s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -51,23 +50,30 @@ __global__ __launch_bounds__(512, 3) void gmm_mx_stream_kernel(MxArgs a)
     s.t1 = EPI == MX_SWIGLU ? s.t0 + tiles / 2 : s.store1 ? s.t0 + 1 : s.t0;
     s.operands(e);
     if (row1 - row0 <= 32) return s.template rows<1, true>(row0, row1);
-    for (int64_t r = row0; r < row1; r += 32) s.template rows<1, false>(r, row1);
+    for (int64_t r = row0 + 32 * blockIdx.z; r < row1; r += 32 * gridDim.z) s.template rows<1, false>(r, row1);
 }
 
 template <int EPI, int DT>
 void launch_stream(const MxArgs& a, hipStream_t st)
 {
     const int64_t pairs = (a.N / 32 + 1) / 2, windows = (a.K + 255) / 256, experts = a.rows < a.E ? a.rows : a.E;
-    int waves = 1;
-    while (waves < 8 && pairs * experts * waves < 256 * 12 && 2 * waves <= windows) waves *= 2;
-    if (const char* s = getenv("MXW")) waves = atoi(s);
-    hipLaunchKernelGGL((gmm_mx_stream_kernel<EPI, DT>), dim3((unsigned)pairs, (unsigned)a.E), dim3(64 * waves),
+    // chunks of 32 rows side by side, twice as many as an expert has on average
+    const int64_t chunks = (2 * a.rows + 32 * a.E - 1) / (32 * a.E), most = (a.rows + 31) / 32, z = chunks < most ? chunks : most;
+    // Wavefronts that share a K: as many as it takes to give every compute unit 12 of them, up to 8 of a window each at least; with
+    // 14 windows and more two or four anyway, since then a workgroup's start is less of it.  us with 1 / 2 / 4: 64 tokens, 256
+    // experts of 7168 -> 2 x 2048 (28 windows) 497 / 493 / 487, of 2048 -> 7168 (8 windows) 258 / 255 / 276; 128 experts of 2048
+    // -> 2 x 768 33.5 / 34.7 / 38.2, one token of it 7.7 / 7.1 / 7.5; a row of 7168 -> 4096 10.9 / 8.1 / 7.4.
+    int waves = windows >= 28 ? 4 : windows >= 14 ? 2 : 1;
+    while (waves < 8 && pairs * experts * z * waves < 256 * 12 && 2 * waves <= windows) waves *= 2;
+    hipLaunchKernelGGL((gmm_mx_stream_kernel<EPI, DT>), dim3((unsigned)pairs, (unsigned)a.E, (unsigned)z), dim3(64 * waves),
                        (waves - 1) * 32 * 64 * 4, st, a);
 }
 
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-int check(const MxArgs& a, bool swiglu)
+}  // namespace
+
+int mx_check(const MxArgs& a, bool swiglu)
 {
     if (a.rows < 0 || a.x_rows < 0 || a.K <= 0 || a.N <= 0 || a.E <= 0) return MOE355_E_ARG;
     if (a.gl_type != MOE355_GL_CUMSUM && a.gl_type != MOE355_GL_COUNT) return MOE355_E_ARG;
@@ -75,20 +81,54 @@ int check(const MxArgs& a, bool swiglu)
         return MOE355_E_SHAPE;
     // rows of x are reached by offsets of 32 bits
     if (a.rows > 0x7fffffff || a.x_rows > 0x7fffffff || a.x_rows * (a.K / 2) > 0xfff00000) return MOE355_E_SHAPE;
+    if (a.rows == 0) return MOE355_OK;
+    if (a.x_rows == 0 || !a.x || !a.x_scale || !a.w || !a.w_scale || (!a.group_list && a.E > 1) || !a.out || (swiglu && !a.out_scale))
+        return MOE355_E_ARG;
+    if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.w_scale, 4) || !aligned(a.out, 16)) return MOE355_E_SHAPE;
     return MOE355_OK;
 }
 
-int run(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)
+MxForm mx_form(int64_t rows, int64_t n, int num_experts, bool swiglu, bool grouped)
 {
-    if (const int rc = check(a, swiglu)) return rc;
-    if (a.rows == 0) return MOE355_OK;
-    if (a.x_rows == 0 || !a.x || !a.x_scale || !a.w || !a.w_scale || (!a.group_list && a.E > 1) || !a.out || (swiglu && !a.out_scale)) return MOE355_E_ARG;
-    if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.w_scale, 4) || !aligned(a.out, 16)) return MOE355_E_SHAPE;
-    if (a.rows >= (getenv("MXT") ? atoi(getenv("MXT")) : 48) * (int64_t)a.E) return launch_mx_tiled(a, swiglu, out_dtype, workspace, workspace_bytes, st);
+    // Streaming has no list to make and splits K, so it is for calls that tiles would not fill the chip with: up to 512 workgroups
+    // of 32 rows x 64 channels, and for fewer than 4 rows an expert.  us streamed / tiles: 8 experts of 1024 -> 2 x 1408, 64 / 128 /
+    // 256 tokens of 2 slots 7.6 / 10.9 / 18.3 against 7.8 / 10.5 / 13.1 (352, 352, 704 workgroups), of 1408 -> 1024 5.1 / - / 6.1
+    // against 6.3 / - / 9.9; one expert of 7168 -> 4096, 128 / 256 / 512 / 1024 rows 10.7 / 19.2 / 30.0 / 57.2 against 26.6 /
+    // 32.3 / 33.7 / 36.5.  128 experts of 2048 -> 2 x 768, 4 / 16 / 64 / 256 tokens of 8 slots 11.8 / 26.5 / 34.6 / 39.5 against
+    // 14.8 / 27.7 / 34.7 / 39.0; skewed (Zipf(1.1)) 64 / 256 tokens 25.0 / 64.4 against 27.2 / 41.3, 256 experts of 7168 -> 2 x
+    // 2048 128 / 512 tokens 249 / 690 against 189 / 317: a hot expert's many rows go through its few workgroups.
+    const int64_t pairs = swiglu ? n / 64 : (n / 32 + 1) / 2, chunks = (rows + 32 * (int64_t)num_experts - 1) / (32 * (int64_t)num_experts);
+    if (rows < 4 * (int64_t)num_experts || pairs * num_experts * chunks <= 512) return MX_STREAM;
+    // Finding the tiles in the product costs a workgroup for every tile that an expert might have, most of which end at once; a
+    // list takes a launch of 5 us in front.  Found / listed, us, at 3 / 6 / 12 / 25 / 33 thousand of them: 34.7 / 35.8 / 39.0
+    // / 50.6 / 38.3 against 38.6 / 39.1 / 41.6 / 54.4 / 32.5, the last two skewed 45.3 / 37.0 against 44.5 / 27.7.
+    const int64_t columns = swiglu ? (n / 64 + 3) / 4 : (n / 32 + 7) / 8, tiles = (rows + kMxTileRows - 1) / kMxTileRows;
+    return grouped && columns * num_experts * tiles > 16384 ? MX_LISTED : MX_TILES;
+}
+
+int mx_launch(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, const MxMap& map, hipStream_t st)
+{
+    if (form != MX_STREAM) return launch_mx_tiled(a, swiglu, out_dtype, form, map, st);
     if (swiglu) launch_stream<MX_SWIGLU, MOE355_DT_BF16>(a, st);
     else if (out_dtype == MOE355_DT_BF16) launch_stream<MX_HALF, MOE355_DT_BF16>(a, st);
     else launch_stream<MX_HALF, MOE355_DT_F16>(a, st);
     return launch_status();
+}
+
+namespace {
+
+int run(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)
+{
+    if (const int rc = mx_check(a, swiglu)) return rc;
+    if (a.rows == 0) return MOE355_OK;
+    const MxForm form = mx_form(a.rows, a.N, a.E, swiglu, a.group_list != nullptr);
+    MxMap map = {};
+    if (form == MX_LISTED) {
+        if (!workspace || !aligned(workspace, 256) || workspace_bytes < mx_map_bytes(a.rows, a.E)) return MOE355_E_WORKSPACE;
+        map = mx_map_in(workspace, a.rows, a.E);
+        mx_build_map(a, map, st);
+    }
+    return mx_launch(a, swiglu, out_dtype, form, map, st);
 }
 
 }  // namespace
@@ -110,10 +150,10 @@ extern "C" int moe355_format_cast_mx(const uint8_t* codes, const uint8_t* scale,
     return launch_status();
 }
 
-extern "C" size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int64_t k, int num_experts)
+extern "C" size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int num_experts, int swiglu)
 {
-    (void)n, (void)k;
-    return rows > 0 && num_experts > 0 ? mx_tiled_workspace(rows, num_experts) : 256;
+    if (rows <= 0 || n <= 0 || num_experts <= 0) return 0;
+    return mx_form(rows, n, num_experts, swiglu != 0, true) == MX_LISTED ? mx_map_bytes(rows, num_experts) : 0;
 }
 
 extern "C" int moe355_gmm_mx(const uint8_t* x, const uint8_t* x_scale, const int32_t* row_token, int64_t x_rows,

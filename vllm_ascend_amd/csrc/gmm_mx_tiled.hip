@@ -12,7 +12,7 @@
 namespace moe355 {
 namespace {
 
-constexpr int kTileRows = 128, kTileTiles = 8;  // tokens, blocks of 32 channels
+constexpr int kTileRows = kMxTileRows;
 constexpr int kThreads = 256;
 constexpr int kRing = 3;
 constexpr int kStage = kTileRows * 128;  // tokens' bytes of a window
@@ -20,18 +20,6 @@ constexpr int kLds = kRing * (kStage + kTileRows * 8);
 
 #define MOE355_GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define MOE355_LPTR(p) ((__attribute__((address_space(3))) void*)(p))
-
-// (expert, rows) of the tiles, in the order of the experts
-struct MxMap {
-    int32_t* count;
-    int32_t *expert, *begin, *end;
-};
-inline int64_t most_tiles(int64_t rows, int E) { return rows / kTileRows + (rows < E ? rows : E); }
-inline MxMap map_in(void* p, int64_t most)
-{
-    int32_t* q = (int32_t*)p;
-    return {q, q + 64, q + 64 + most, q + 64 + 2 * most};
-}
 
 // One workgroup; thread t has the experts [t seg, (t + 1) seg).  Rows are cut to those that exist.
 __global__ __launch_bounds__(1024) void mx_map_kernel(const int64_t* __restrict__ list, int gl_type, int E, int64_t rows, MxMap map,
@@ -98,7 +86,7 @@ __global__ __launch_bounds__(1024) void mx_map_kernel(const int64_t* __restrict_
     }
 }
 
-template <int EPI, int DT>
+template <int EPI, int DT, bool LISTED>
 __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxMap map)
 {
     // (not an array of a known size: the compiler would wait for every load on its way to it before each read)
@@ -109,14 +97,29 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const int tiles = (int)(a.N / 32), steps = (int)(a.K / 64), windows = (steps + 3) / 4;
     const int columns = EPI == MX_SWIGLU ? (tiles / 2 + 3) / 4 : (tiles + 7) / 8;
 
-    // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one after
-    // the other, so that the tile's tokens and the expert's weights stay in its L2.
-    const int64_t count = a.group_list ? map.count[0] : (a.rows + kTileRows - 1) / kTileRows;
-    const int64_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
-    if ((int64_t)(blockIdx.x >> 3) >= share || item >= items) return;
-    const int tile = (int)(item / columns), column = (int)(item % columns);
-    const int e = a.group_list ? map.expert[tile] : 0;
-    const int64_t row0 = a.group_list ? map.begin[tile] : (int64_t)tile * kTileRows, row1 = a.group_list ? map.end[tile] : a.rows;
+    int e, column;
+    int64_t row0, row1;
+    if (LISTED || !a.group_list) {
+        // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one
+        // after the other, so that the tile's tokens and the expert's weights stay in its L2.
+        const uint32_t count = LISTED ? map.count[0] : (uint32_t)((a.rows + kTileRows - 1) / kTileRows);
+        const uint32_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= share || item >= items) return;
+        const int tile = (int)(item / columns);
+        column = (int)(item - tile * columns);
+        e = LISTED ? map.expert[tile] : 0;
+        row0 = LISTED ? map.begin[tile] : (int64_t)tile * kTileRows;
+        row1 = LISTED ? map.end[tile] : a.rows;
+    } else {
+        // (column, expert, tile of it): most experts have fewer tiles than they might
+        column = blockIdx.x;
+        e = blockIdx.y;
+        const int64_t n = a.group_list[e], m = a.gl_type == MOE355_GL_CUMSUM ? n - (e > 0 ? a.group_list[e - 1] : 0) : n;
+        if (m <= (int64_t)blockIdx.z * kTileRows) return;
+        mx_expert_rows(a, e, lane, row0, row1);
+        row0 += (int64_t)blockIdx.z * kTileRows;
+        if (row0 >= row1) return;
+    }
 
     // this wavefront's two blocks of channels (a block past the last one computes the last one again and is not stored)
     const int b0 = EPI == MX_SWIGLU ? column * 4 + wave : column * 8 + 2 * wave;
@@ -137,8 +140,8 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const auto ws0 = mx_buffer(a.w_scale + ((int64_t)e * tiles + t0) * windows * 256, windows * 256);
     const auto ws1 = mx_buffer(a.w_scale + ((int64_t)e * tiles + t1) * windows * 256, windows * 256);
 
-    // Tokens' bytes of a window: row-major, 128 bytes a row, the 16-byte pieces exchanged by row so that the 8 lanes that LDS
-    // serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.
+    // Tokens' bytes of a window: row-major, 128 bytes a row, the 16-byte pieces exchanged by row pair so that the 16 lanes that
+    // LDS serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.
     auto token_of = [&](int64_t row) -> uint32_t {
         row = row < row1 ? row : row1 - 1;  // rows behind the last one are not stored
         if (!a.row_token) return (uint32_t)row;
@@ -147,19 +150,22 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     };
     const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
     uint32_t from[4];
-    const int piece = (lane & 7) ^ (lane >> 3);
+    const int piece = (lane & 7) ^ (lane >> 4);  // of rows 8 i + lane / 8 with even i; with odd ones piece ^ 4
 #pragma unroll
-    for (int i = 0; i < 4; ++i) from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + piece * 16;
+    for (int i = 0; i < 4; ++i)
+        from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16;
     // scales: thread t has row t / 2, half t % 2
     const uint32_t scale_from = token_of(row0 + (threadIdx.x >> 1)) * (uint32_t)(a.K / 32);
 
     auto fetch_tokens = [&](int w, int slot) {
         // a shorter last window has 32 bytes a step of a row; the pieces behind them are the first one again (not used)
-        const uint32_t back = w < full || piece < 2 * tail ? 0 : piece * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            const int p = piece ^ (i & 1) * 4;
+            const uint32_t back = w < full || p < 2 * tail ? 0 : p * 16;
             __builtin_amdgcn_global_load_lds(MOE355_GPTR(a.x + w * 128 + (from[i] - back)),
                                              MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16, 0, 0);
+        }
     };
     const uint32_t scale_end = mx_scale_bytes(a) - 4;
     const auto x_scales = mx_buffer(a.x_scale, scale_end + 4);
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         for (int t = 0; t < 4; ++t) sb[t] = scales[slot * (2 * kTileRows) + (t * 32 + row_in) * 2 + half];
         const uint8_t* base = tokens + slot * kStage + row_in * 128;
         v4i b[4];
-        auto read = [&](int j, int t) { b[t] = *(const v4i*)(base + t * 32 * 128 + ((half * nb + j) ^ (row_in & 7)) * 16); };
+        auto read = [&](int j, int t) { b[t] = *(const v4i*)(base + t * 32 * 128 + ((half * nb + j) ^ (row_in >> 1 & 7)) * 16); };
 #pragma unroll
         for (int t = 0; t < 4; ++t) read(0, t);
         // the next step's tokens into the registers that this step's products have just used, six products ahead
@@ -245,6 +251,8 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         __builtin_amdgcn_sched_barrier(0);
         slot = slot1;
     };
+    // products before the vector instructions of the other workgroup's prologue and epilogue
+    __builtin_amdgcn_s_setprio(1);
     constexpr std::true_type whole{};
     constexpr std::false_type part{};
     int w = 0;
@@ -257,6 +265,7 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         held[0] = held[1];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end still write LDS
+    __builtin_amdgcn_s_setprio(0);
 
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -286,28 +295,42 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
 
 }  // namespace
 
-size_t mx_tiled_workspace(int64_t rows, int num_experts)
+size_t mx_map_bytes(int64_t rows, int num_experts)
 {
-    return (size_t)((64 + 3 * most_tiles(rows, num_experts)) * 4 + 255) / 256 * 256;
+    return (size_t)((64 + 3 * mx_most_tiles(rows, num_experts)) * 4 + 255) / 256 * 256;
 }
 
-int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, void* workspace, size_t workspace_bytes, hipStream_t st)
+MxMap mx_map_in(void* workspace, int64_t rows, int num_experts)
 {
-    const int64_t most = a.group_list ? most_tiles(a.rows, a.E) : (a.rows + kTileRows - 1) / kTileRows;
-    const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, groups = (most * columns + 7) / 8 * 8;
+    int32_t* q = (int32_t*)workspace;
+    const int64_t most = mx_most_tiles(rows, num_experts);
+    return {q, q + 64, q + 64 + most, q + 64 + 2 * most};
+}
+
+void mx_build_map(const MxArgs& a, const MxMap& map, hipStream_t st)
+{
+    hipLaunchKernelGGL(mx_map_kernel, dim3(1), dim3(1024), 0, st, a.group_list, a.gl_type, a.E, a.rows, map,
+                       (int32_t)mx_most_tiles(a.rows, a.E));
+}
+
+int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, const MxMap& map, hipStream_t st)
+{
+    const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, tiles = (a.rows + kTileRows - 1) / kTileRows;
+    const int64_t most = form == MX_LISTED ? mx_most_tiles(a.rows, a.E) : tiles, groups = (most * columns + 7) / 8 * 8;
     if (groups > 0x7fffffff) return MOE355_E_SHAPE;
-    MxMap map = {};
-    if (a.group_list) {
-        if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < mx_tiled_workspace(a.rows, a.E))
-            return MOE355_E_WORKSPACE;
-        map = map_in(workspace, most);
-        hipLaunchKernelGGL(mx_map_kernel, dim3(1), dim3(1024), 0, st, a.group_list, a.gl_type, a.E, a.rows, map, (int32_t)most);
-    }
-    const dim3 grid((unsigned)groups);
-    if (swiglu) hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_SWIGLU, MOE355_DT_BF16>), grid, dim3(kThreads), kLds, st, a, map);
-    else if (out_dtype == MOE355_DT_BF16)
-        hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_HALF, MOE355_DT_BF16>), grid, dim3(kThreads), kLds, st, a, map);
-    else hipLaunchKernelGGL((gmm_mx_tiled_kernel<MX_HALF, MOE355_DT_F16>), grid, dim3(kThreads), kLds, st, a, map);
+    const bool direct = form == MX_TILES && a.group_list;
+    const dim3 grid = direct ? dim3((unsigned)columns, (unsigned)a.E, (unsigned)tiles) : dim3((unsigned)groups);
+#define MOE355_MXT(E_, D_)                                                                                       \
+    do {                                                                                                         \
+        if (form == MX_LISTED)                                                                                   \
+            hipLaunchKernelGGL((gmm_mx_tiled_kernel<E_, D_, true>), grid, dim3(kThreads), kLds, st, a, map);     \
+        else                                                                                                     \
+            hipLaunchKernelGGL((gmm_mx_tiled_kernel<E_, D_, false>), grid, dim3(kThreads), kLds, st, a, map);    \
+    } while (0)
+    if (swiglu) MOE355_MXT(MX_SWIGLU, MOE355_DT_BF16);
+    else if (out_dtype == MOE355_DT_BF16) MOE355_MXT(MX_HALF, MOE355_DT_BF16);
+    else MOE355_MXT(MX_HALF, MOE355_DT_F16);
+#undef MOE355_MXT
     return launch_status();
 }
 

@@ -852,17 +852,17 @@ def w4_offset_correction(weight_nz4, weight_scale, group_size, n, k):
 MX_BLOCK = 32  # values that share a scale
 
 
-def _bytes(t: torch.Tensor, name: str, kinds=("float4_e2m1fn_x2",)) -> torch.Tensor:
+def _bytes(t: torch.Tensor, name: str, kind: str = "float4_e2m1fn_x2") -> torch.Tensor:
     """Codes or E8M0 scales as uint8, under whichever of their names they come."""
-    if t.dtype == torch.uint8:
+    if t.dtype is torch.uint8:
         return t
-    if any(t.dtype == getattr(torch, kind, None) for kind in kinds):
+    if t.dtype == getattr(torch, kind, None):
         return t.view(torch.uint8)
-    raise TypeError(f"{name}: uint8 or {' or '.join(kinds)} tensor expected but got {t.dtype}")
+    raise TypeError(f"{name}: uint8 or {kind} tensor expected but got {t.dtype}")
 
 
 def _scale_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
-    return _bytes(t, name, ("float8_e8m0fnu",))
+    return _bytes(t, name, "float8_e8m0fnu")
 
 
 def _flat(t: torch.Tensor, name: str, alignment: int = 16) -> torch.Tensor:
@@ -871,26 +871,29 @@ def _flat(t: torch.Tensor, name: str, alignment: int = 16) -> torch.Tensor:
     return t if t.data_ptr() % alignment == 0 else t.clone()
 
 
-def _call(device: torch.device, name: str, *args) -> None:
+def _call(index: int, name: str, *args) -> None:
     """An entry point of the library on torch's current stream of a device, which need not be the current device."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, _raw_stream(device.index)), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _raw_stream(device.index)), name)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
 
 
-def _on(x: torch.Tensor, **others) -> None:
+def _on(index: int, **others) -> None:
     for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{name} is on {t.device}, the rows on {x.device}")
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"{name} is on {t.device}, the rows on device {index}")
 
 
 def _rows_of(x: torch.Tensor, op: str, multiple: int) -> tuple[int, int]:
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % multiple:
-        raise ValueError(f"{op}: rows must hold a multiple of {multiple} values, got {tuple(x.shape)}")
-    return x.numel() // x.shape[-1], x.shape[-1]
+    shape = x.shape
+    if not shape or shape[-1] == 0 or shape[-1] % multiple:
+        raise ValueError(f"{op}: rows must hold a multiple of {multiple} values, got {tuple(shape)}")
+    return x.numel() // shape[-1], shape[-1]
 
 
 def dynamic_mx_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -898,9 +901,10 @@ def dynamic_mx_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dt = _dt(x, "x")
     rows, cols = _rows_of(x, "dynamic_mx_quant", MX_BLOCK)
     x = _flat(x, "x")
-    codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((*x.shape[:-1], cols // MX_BLOCK), dtype=torch.uint8, device=x.device)
-    _call(x.device, "moe355_dynamic_mx_quant", _ptr(x), dt, rows, cols, _ptr(codes), _ptr(scale))
+    lead = x.shape[:-1]
+    codes = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((*lead, cols // MX_BLOCK), dtype=torch.uint8, device=x.device)
+    _call(x.get_device(), "moe355_dynamic_mx_quant", x.data_ptr(), dt, rows, cols, codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -910,12 +914,14 @@ def mx_dequant(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = to
         raise TypeError(f"mx_dequant: float16, float32 or bfloat16 output expected but got {dtype}")
     codes, scale = _bytes(codes, "codes"), _scale_bytes(scale, "scale")
     rows, half = _rows_of(codes, "mx_dequant", MX_BLOCK // 2)
-    if scale.shape != (*codes.shape[:-1], half * 2 // MX_BLOCK):
+    lead = codes.shape[:-1]
+    if scale.shape != (*lead, half * 2 // MX_BLOCK):
         raise ValueError(f"mx_dequant: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
     codes, scale = _flat(codes, "codes", 4), _dev(scale, "scale")
-    _on(codes, scale=scale)
-    out = torch.empty((*codes.shape[:-1], half * 2), dtype=dtype, device=codes.device)
-    _call(codes.device, "moe355_mx_dequant", _ptr(codes), _ptr(scale), rows, half * 2, _ptr(out), _DT[dtype])
+    index = codes.get_device()
+    _on(index, scale=scale)
+    out = torch.empty((*lead, half * 2), dtype=dtype, device=codes.device)
+    _call(index, "moe355_mx_dequant", codes.data_ptr(), scale.data_ptr(), rows, half * 2, out.data_ptr(), _DT[dtype])
     return out
 
 
@@ -923,14 +929,14 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
     """x = x1 (+ x2), y = RMS norm of x, q and scale = y quantised: int8 with an fp32 scale a row (``NORM_INT8``), MXFP4
     (``NORM_MXFP4``) or not at all (``NORM_PLAIN``: None, None).  -> (q, scale, y, x); without x2, x is x1 itself."""
     op = "add_rms_norm_quant"
-    dt = _dt(x1, "x1")
-    _half_dtype(x1.dtype)
+    dtype = _half_dtype(x1.dtype)
     rows, cols = _rows_of(x1, op, MX_BLOCK if kind == NORM_MXFP4 else 8)
-    if x2 is not None and (x2.shape != x1.shape or x2.dtype != x1.dtype):
-        raise ValueError(f"{op}: x2 {tuple(x2.shape)} {x2.dtype} does not match x1 {tuple(x1.shape)} {x1.dtype}")
-    if gamma.dtype not in (x1.dtype, torch.float32) or gamma.shape != (cols,):
-        raise ValueError(f"{op}: gamma must hold {cols} values of {x1.dtype} or float32, got {tuple(gamma.shape)} "
-                         f"{gamma.dtype}")
+    lead = x1.shape[:-1]
+    if x2 is not None and (x2.shape != x1.shape or x2.dtype != dtype):
+        raise ValueError(f"{op}: x2 {tuple(x2.shape)} {x2.dtype} does not match x1 {tuple(x1.shape)} {dtype}")
+    wide = gamma.dtype is torch.float32
+    if not (wide or gamma.dtype is dtype) or gamma.shape != (cols,):
+        raise ValueError(f"{op}: gamma must hold {cols} values of {dtype} or float32, got {tuple(gamma.shape)} {gamma.dtype}")
     if beta is not None and (beta.dtype != gamma.dtype or beta.shape != gamma.shape):
         raise ValueError(f"{op}: beta {tuple(beta.shape)} {beta.dtype} does not match gamma {tuple(gamma.shape)} "
                          f"{gamma.dtype}")
@@ -938,8 +944,8 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
     x1 = _flat(x1, "x1")
     x2 = None if x2 is None else _flat(x2, "x2")
     gamma, beta = _flat(gamma, "gamma"), None if beta is None else _flat(beta, "beta")
-    _on(x1, x2=x2, gamma=gamma, beta=beta)
-    dev, lead = x1.device, x1.shape[:-1]
+    index, dev = x1.get_device(), x1.device
+    _on(index, x2=x2, gamma=gamma, beta=beta)
     y = torch.empty_like(x1)
     x = torch.empty_like(x1) if x2 is not None else None
     q = scale = None
@@ -949,8 +955,9 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
     elif kind == NORM_MXFP4:
         q = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
         scale = torch.empty((*lead, cols // MX_BLOCK), dtype=torch.uint8, device=dev)
-    _call(dev, "moe355_add_rms_norm_quant", _ptr(x1), _ptr(x2), _ptr(gamma), _ptr(beta), dt, _dt(gamma, "gamma"), rows,
-          cols, float(epsilon), kind, _ptr(x), _ptr(y), _ptr(q), _ptr(scale))
+    dt = _DT[dtype]
+    _call(index, "moe355_add_rms_norm_quant", x1.data_ptr(), _ptr(x2), gamma.data_ptr(), _ptr(beta), dt, DT_F32 if wide else dt,
+          rows, cols, epsilon, kind, _ptr(x), y.data_ptr(), _ptr(q), _ptr(scale))
     return q, scale, y, given if x is None else x
 
 
@@ -971,74 +978,133 @@ def format_cast_mx(codes: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tens
     if scale.shape != (E, n, k // MX_BLOCK):
         raise ValueError(f"format_cast_mx: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
     codes, scale = _flat(codes, "weight"), _dev(scale, "scale")
-    _on(codes, scale=scale)
+    _on(codes.get_device(), scale=scale)
     out = torch.empty_like(codes)
     out_scale = torch.empty((E, n, mx_scale_columns(k)), dtype=torch.uint8, device=codes.device)
-    _call(codes.device, "moe355_format_cast_mx", _ptr(codes), _ptr(scale), E, n, k, _ptr(out), _ptr(out_scale))
+    _call(codes.get_device(), "moe355_format_cast_mx", codes.data_ptr(), scale.data_ptr(), E, n, k, out.data_ptr(),
+          out_scale.data_ptr())
     return out, out_scale
 
 
-def _mx_operands(op, x, x_scale, weight, weight_scale, group_list, row_map, n_multiple):
-    """The checks of the products; -> contiguous operands and (rows, n, k, E)."""
-    x, x_scale = _bytes(x, "x"), _scale_bytes(x_scale, "x_scale")
+def _mx_weights(op, weight, weight_scale, n_multiple):
+    """-> laid-out weights and scales, E, n, k"""
     weight, weight_scale = _bytes(weight, "weight"), _scale_bytes(weight_scale, "weight_scale")
-    if weight.dim() != 3:
-        raise ValueError(f"{op}: weight must be [E, N, K / 2] (format_cast_mx), got {tuple(weight.shape)}")
-    E, n, k = weight.shape[0], weight.shape[1], weight.shape[2] * 2
-    if n % n_multiple or k % 64 or not weight.numel():
+    shape = weight.shape
+    if len(shape) != 3:
+        raise ValueError(f"{op}: weight must be [E, N, K / 2] (format_cast_mx), got {tuple(shape)}")
+    E, n, k = shape[0], shape[1], shape[2] * 2
+    if not E or not n or not k or n % n_multiple or k % 64:
         raise ValueError(f"{op}: N must be a multiple of {n_multiple} and K of 64, got E = {E}, N = {n}, K = {k}")
     if weight_scale.shape != (E, n, mx_scale_columns(k)):
         raise ValueError(f"{op}: weight_scale must be {(E, n, mx_scale_columns(k))} (format_cast_mx), got "
                          f"{tuple(weight_scale.shape)}")
-    if x.dim() != 2 or x.shape[1] * 2 != k:
-        raise ValueError(f"{op}: x must be [rows, K / 2 = {k // 2}], got {tuple(x.shape)}")
-    if x_scale.shape != (x.shape[0], k // MX_BLOCK):
-        raise ValueError(f"{op}: x_scale must be {(x.shape[0], k // MX_BLOCK)}, got {tuple(x_scale.shape)}")
+    return weight, weight_scale, E, n, k
+
+
+def _mx_rows(op, x, x_scale, k):
+    x, x_scale = _bytes(x, "x"), _scale_bytes(x_scale, "x_scale")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] * 2 != k:
+        raise ValueError(f"{op}: x must be [rows, K / 2 = {k // 2}], got {tuple(shape)}")
+    if x_scale.shape != (shape[0], k // MX_BLOCK):
+        raise ValueError(f"{op}: x_scale must be {(shape[0], k // MX_BLOCK)}, got {tuple(x_scale.shape)}")
+    if k == 64 and shape[0] == 1:
+        x_scale = torch.nn.functional.pad(x_scale.reshape(-1), (0, 2))  # the kernels read four scales at a time
+    return x, x_scale
+
+
+def _mx_product(op, entry, x, x_scale, weight, weight_scale, group_list, group_list_type, row_map, swiglu):
+    """What the two products have in common: -> (n, the call that writes given outputs, rows, device)"""
+    weight, weight_scale, E, n, k = _mx_weights(op, weight, weight_scale, 64 if swiglu else 32)
+    x, x_scale = _mx_rows(op, x, x_scale, k)
+    x_rows = rows = x.shape[0]
     if group_list is None:
         if E != 1:
             raise ValueError(f"{op}: {E} experts need a group_list")
     elif group_list.dim() != 1 or group_list.numel() != E or group_list.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{op}: group_list must hold one integer per expert ({E}), got {tuple(group_list.shape)} "
                          f"{group_list.dtype}")
-    rows = x.shape[0]
     if row_map is not None:
         if row_map.dtype != torch.int32 or row_map.dim() != 1:
             raise TypeError(f"{op}: row_map must be a vector of int32, got {tuple(row_map.shape)} {row_map.dtype}")
-        rows, row_map = row_map.numel(), _dev(row_map, "row_map")
-        if rows and not x.shape[0]:
+        rows = row_map.numel()
+        if rows and not x_rows:
             raise ValueError(f"{op}: row_map names {rows} rows of an empty x")
+        row_map = _dev(row_map, "row_map")
     x, x_scale = _flat(x, "x"), _dev(x_scale, "x_scale")
-    if x_scale.numel() < 4:
-        x_scale = torch.nn.functional.pad(x_scale.reshape(-1), (0, 4 - x_scale.numel()))  # the kernels read four at a time
     weight, weight_scale = _flat(weight, "weight"), _flat(weight_scale, "weight_scale")
-    group_list = None if group_list is None else _gl(group_list)
-    _on(x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, row_map=row_map)
-    return x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E
+    if group_list is not None:
+        group_list = _gl(group_list)
+    index = x.get_device()
+    _on(index, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, row_map=row_map)
+    list_type = _gl_type(group_list_type)
+
+    def call(*outputs):
+        nbytes = 0 if group_list is None else _lib.load().moe355_gmm_mx_workspace(rows, n, E, swiglu)
+        ws = _workspace(nbytes, x.device) if nbytes else None
+        _call(index, entry, x.data_ptr(), x_scale.data_ptr(), _ptr(row_map), x_rows, weight.data_ptr(), weight_scale.data_ptr(),
+              _ptr(group_list), list_type, rows, k, n, E, *outputs, _ptr(ws), nbytes)
+
+    return n, call, rows, x.device
 
 
 def gmm_mx(x, x_scale, weight, weight_scale, group_list, group_list_type, out_dtype=torch.bfloat16, row_map=None):
     """MXFP4 rows [M, K / 2] times their experts' weights [E, N, K / 2] -> 16-bit [rows, N].  row_map: the row of x of every
     sorted row; without it the rows of x are sorted by expert.  group_list None: one expert, which has all rows."""
-    x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E = _mx_operands(
-        "gmm_mx", x, x_scale, weight, weight_scale, group_list, row_map, 32)
-    out = torch.empty((rows, n), dtype=_half_dtype(out_dtype), device=x.device)
-    lib = _lib.load()
-    ws = _workspace(lib.moe355_gmm_mx_workspace(rows, n, k, E), x.device)
-    _call(x.device, "moe355_gmm_mx", _ptr(x), _ptr(x_scale), _ptr(row_map), x.shape[0], _ptr(weight),
-          _ptr(weight_scale), _ptr(group_list), _gl_type(group_list_type), rows, k, n, E, _ptr(out), _dt(out, "out"),
-          _ptr(ws), ws.numel())
+    n, call, rows, device = _mx_product("gmm_mx", "moe355_gmm_mx", x, x_scale, weight, weight_scale, group_list, group_list_type,
+                                        row_map, 0)
+    out = torch.empty((rows, n), dtype=_half_dtype(out_dtype), device=device)
+    call(out.data_ptr(), _DT[out_dtype])
     return out
 
 
 def gmm_mx_swiglu_quant(x, x_scale, weight, weight_scale, group_list, group_list_type, swiglu_limit=0.0, row_map=None):
     """... with the gate_up weights [E, 2 I, K / 2], through SwiGLU to MXFP4: (codes [rows, I / 2], scales [rows, I / 32])."""
-    x, x_scale, weight, weight_scale, group_list, row_map, rows, n, k, E = _mx_operands(
-        "gmm_mx_swiglu_quant", x, x_scale, weight, weight_scale, group_list, row_map, 64)
-    out = torch.empty((rows, n // 4), dtype=torch.uint8, device=x.device)
-    out_scale = torch.empty((rows, n // 64), dtype=torch.uint8, device=x.device)
-    lib = _lib.load()
-    ws = _workspace(lib.moe355_gmm_mx_workspace(rows, n, k, E), x.device)
-    _call(x.device, "moe355_gmm_mx_swiglu_quant", _ptr(x), _ptr(x_scale), _ptr(row_map), x.shape[0], _ptr(weight),
-          _ptr(weight_scale), _ptr(group_list), _gl_type(group_list_type), rows, k, n, E, float(swiglu_limit),
-          _ptr(out), _ptr(out_scale), _ptr(ws), ws.numel())
+    n, call, rows, device = _mx_product("gmm_mx_swiglu_quant", "moe355_gmm_mx_swiglu_quant", x, x_scale, weight, weight_scale,
+                                        group_list, group_list_type, row_map, 1)
+    out = torch.empty((rows, n // 4), dtype=torch.uint8, device=device)
+    out_scale = torch.empty((rows, n // 64), dtype=torch.uint8, device=device)
+    call(swiglu_limit, out.data_ptr(), out_scale.data_ptr())
     return out, out_scale
+
+
+def mx_experts(x, x_scale, topk_ids, topk_weights, w13, w13_scale, w2, w2_scale, swiglu_limit=0.0, residual=None):
+    """All MXFP4 experts on tokens whose routing is known, in one native call: dynamic_mx_quant (x_scale None: x [T, H] in 16 bits;
+    otherwise x [T, H / 2] and x_scale are the quantised rows), route_map, gmm_mx_swiglu_quant, gmm_mx, token_unpermute.  The
+    result has the dtype of topk_weights.  -> (out [T, H], expert_tokens [E])"""
+    op = "mx_experts"
+    w13, w13_scale, E, two_i, H = _mx_weights(op, w13, w13_scale, 64)
+    w2, w2_scale, E2, h, I = _mx_weights(op, w2, w2_scale, 32)
+    if E2 != E or h != H or 2 * I != two_i:
+        raise ValueError(f"{op}: w13 is [{E}, {two_i}, K = {H}], w2 [{E2}, {h}, K = {I}]")
+    dtype = _half_dtype(topk_weights.dtype)
+    if x_scale is None:
+        if x.dtype is not dtype or x.dim() != 2 or x.shape[1] != H:
+            raise ValueError(f"{op}: x must be [T, {H}] of {dtype}, got {tuple(x.shape)} {x.dtype}")
+    else:
+        x, x_scale = _mx_rows(op, x, x_scale, H)
+    T = x.shape[0]
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != T or topk_weights.shape != topk_ids.shape:
+        raise ValueError(f"{op}: {T} tokens, but topk_ids {tuple(topk_ids.shape)} and topk_weights {tuple(topk_weights.shape)}")
+    if topk_ids.dtype is not torch.int32:
+        topk_ids = topk_ids.to(torch.int32)
+    if residual is not None:
+        if residual.dtype != dtype or residual.shape != (T, H):
+            raise ValueError(f"{op}: residual must be {dtype} of shape {(T, H)}, got {residual.dtype} {tuple(residual.shape)}")
+        residual = _flat(residual, "residual")
+    x, x_scale = _flat(x, "x"), None if x_scale is None else _dev(x_scale, "x_scale")
+    w13, w13_scale = _flat(w13, "w13"), _flat(w13_scale, "w13_scale")
+    w2, w2_scale, index = _flat(w2, "w2"), _flat(w2_scale, "w2_scale"), x.get_device()
+    topk_ids, topk_weights = _dev(topk_ids, "topk_ids"), _dev(topk_weights, "topk_weights")
+    _on(index, x_scale=x_scale, topk_ids=topk_ids, topk_weights=topk_weights, w13=w13, w13_scale=w13_scale, w2=w2,
+        w2_scale=w2_scale, residual=residual)
+    k, dev = topk_ids.shape[1], x.device
+    out = torch.empty((T, H), dtype=dtype, device=dev)
+    tokens = (torch.empty if T else torch.zeros)((E,), dtype=torch.int64, device=dev)
+    if T:
+        nbytes = _lib.load().moe355_mx_experts_workspace(T, k, H, I, E, int(x_scale is not None))
+        ws = _workspace(nbytes, dev)
+        _call(index, "moe355_mx_experts", x.data_ptr(), _ptr(x_scale), _DT[dtype], T, H, topk_ids.data_ptr(),
+              topk_weights.data_ptr(), k, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), I, E,
+              swiglu_limit, _ptr(residual), tokens.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
+    return out, tokens

@@ -63,42 +63,49 @@ class AscendW4A4MXFP4DynamicFusedMoEMethod(AscendMoEScheme):
         scales in ``layer.ascend_pertoken_scale``).  The rows stay in token order: the gate_up product reads them through
         the row -> token map of the routing."""
         self._refuse(layer)
-        if topk_ids.dim() != 2:
-            raise ValueError(f"topk_ids must be [T, k], got {tuple(topk_ids.shape)}")
-        stream = torch.cuda.current_stream()
-        before_dispatch_evt = stream.record_event()
-        scale = getattr(layer, "ascend_pertoken_scale", None)
-        given = scale is not None
-        if given:
-            codes = kernels._bytes(x, "hidden states quantised by the caller")
-        else:
+        scale = layer.ascend_pertoken_scale
+        if scale is None:
             if x.dtype != self.in_dtype:
                 raise TypeError(f"hidden states are {x.dtype}, the scheme was built for {self.in_dtype}")
-            codes, scale = npu_ops.npu_dynamic_mx_quant(x)
-        lead, H = x.shape[:-1], codes.shape[-1] * 2
-        codes, scale = codes.reshape(-1, codes.shape[-1]), scale.reshape(-1, scale.shape[-1])
-        if topk_ids.shape[0] != codes.shape[0] or topk_weights.shape != topk_ids.shape:
-            raise ValueError(f"{codes.shape[0]} tokens, but topk_ids {tuple(topk_ids.shape)} and topk_weights "
+            H = x.shape[-1]
+        else:
+            x = kernels._bytes(x, "hidden states quantised by the caller")
+            H = x.shape[-1] * 2
+            if x.dim() != 2:
+                scale = scale.reshape(-1, scale.shape[-1])
+        lead = x.shape[:-1]
+        if x.dim() != 2:
+            x = x.reshape(-1, x.shape[-1])
+        if topk_weights.dtype != self.in_dtype:
+            topk_weights = topk_weights.to(self.in_dtype)
+        if topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0] or topk_weights.shape != topk_ids.shape:
+            raise ValueError(f"{x.shape[0]} tokens, but topk_ids {tuple(topk_ids.shape)} and topk_weights "
                              f"{tuple(topk_weights.shape)}")
-        shared_out = None
-        if shared_experts is not None:
-            if shared_experts_input is None:
-                shared_experts_input = npu_ops.npu_mx_dequant(codes, scale, dst_type=self.in_dtype) if given else x
-            shared_out = shared_experts(shared_experts_input)
-        limit = getattr(getattr(layer, "moe_config", None), "swiglu_limit", 0.0) or 0.0
+        limit = layer.moe_config.swiglu_limit or 0.0
+        if shared_experts is None:
+            # one native call; no events are recorded, which are for what runs beside the routed experts
+            out, expert_tokens = kernels.mx_experts(x, scale, topk_ids, topk_weights, layer.w13_weight, layer.w13_weight_scale,
+                                                    layer.w2_weight, layer.w2_weight_scale, limit)
+            return FusedExpertsResult(routed_out=out if len(lead) == 1 else out.reshape(*lead, H), group_list_type=1,
+                                      expert_tokens=expert_tokens)
+        stream = torch.cuda.current_stream()
+        before_dispatch_evt = stream.record_event()
+        if shared_experts_input is None:
+            shared_experts_input = x if scale is None else npu_ops.npu_mx_dequant(x, scale, dst_type=self.in_dtype)
+        shared_out = shared_experts(shared_experts_input)
+        if scale is None:
+            x, scale = npu_ops.npu_dynamic_mx_quant(x)
         expanded_row_idx, row_token, expert_tokens = kernels.route_map(topk_ids, layer.w13_weight.shape[0], 1)
         hidden, hidden_scale = npu_ops.npu_grouped_matmul_swiglu_quant_v2(
-            codes, layer.w13_weight, layer.w13_weight_scale, scale, expert_tokens, group_list_type=1, swiglu_limit=limit,
+            x, layer.w13_weight, layer.w13_weight_scale, scale, expert_tokens, group_list_type=1, swiglu_limit=limit,
             row_map=row_token)
         before_gmm2_evt = stream.record_event()
         out = npu_ops.npu_grouped_matmul([hidden], [layer.w2_weight], scale=[layer.w2_weight_scale],
                                          per_token_scale=[hidden_scale], group_list=expert_tokens, split_item=2,
                                          group_type=0, group_list_type=1, output_dtype=self.in_dtype)[0]
         before_combine_evt = stream.record_event()
-        if shared_out is not None:
-            shared_experts.wait()
-            shared_out = shared_out.reshape(-1, H)
-        routed_out = kernels.token_unpermute(out, expanded_row_idx, topk_weights.to(self.in_dtype), shared_out)
+        shared_experts.wait()
+        routed_out = kernels.token_unpermute(out, expanded_row_idx, topk_weights, shared_out.reshape(-1, H))
         return FusedExpertsResult(routed_out=routed_out.reshape(*lead, H), before_dispatch_evt=before_dispatch_evt,
                                   before_gmm2_evt=before_gmm2_evt, before_combine_evt=before_combine_evt,
                                   group_list_type=1, expert_tokens=expert_tokens, shared_out=shared_out)
