@@ -22,6 +22,12 @@
 
 namespace moe355 {
 
+// 16 bytes written through the L2 (gmm_common.h measures what that does for the outputs of large products)
+__device__ __forceinline__ void store16_through(void* p, v4i v)
+{
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
+}
+
 struct MxArgs {
     const uint8_t* x;           // [x_rows, K / 2] codes
     const uint8_t* x_scale;     // [x_rows, K / 32]
@@ -35,9 +41,14 @@ struct MxArgs {
     float limit;                // SwiGLU's clamp
     void* out;                  // 16-bit [rows, N], or codes [rows, N / 4] of the N / 2 values of SwiGLU
     uint8_t* out_scale;         // [rows, N / 64]
+    bool far;                   // the 16-bit output is larger than the last cache
 };
 
 enum { MX_HALF = 0, MX_SWIGLU = 1 };
+
+// A 16-bit output that the 256 MiB of the last cache do not hold is stored past it: 65536 rows of 768 -> 2048, 268 MB, 129 -> 107 us
+// (half as many rows: no difference, and what reads them next finds them there).
+inline bool mx_far(int64_t rows, int64_t n) { return rows * n >= (int64_t)96 << 20; }
 
 __device__ __forceinline__ v16f mfma_mx(v4i a, v4i b, v16f c, int sa, int sb, int j)
 {
@@ -107,8 +118,13 @@ __device__ __forceinline__ float swiglu_f64(float g, float u)
     return (float)(d / (1.0 + exp(-d)) * (double)u);
 }
 
-// A block of 32 output channels of a token, of which this lane has 16: silu(gate) * up to MXFP4, codes 16 bytes at `codes`, its
-// scale at `scale`.  Both halves of the wavefront call it together; `store`: whether the lane's token exists.
+// A block of 32 output channels of a token, of which this lane has 16: silu(gate) * up to MXFP4, codes of channels 0-15 in the
+// lower half of the wavefront, of 16-31 in the upper one, the scale in both.  Both halves call it together; `exists`: whether the
+// lane's token does.
+struct MxBlock {
+    uint2 codes;
+    uint32_t scale;
+};
 //
 // What is quantised is the value of the formula, rounded to binary32.  The hardware's exp2 and reciprocal make it in 13 issue
 // slots a value (a transcendental instruction takes four; the IEEE sequence of the int8 epilogues takes 30), off by at most
@@ -117,7 +133,7 @@ __device__ __forceinline__ float swiglu_f64(float g, float u)
 // which have a mantissa of two bits and then zeros.  A value within 64 units of such a number (6 in 10^5 of them; infinities
 // and NaN look like one) is computed again in 64 bits, and so is one with a gate below -32, unless it is small enough beside its
 // block to have the code of zero anyway.  The codes are therefore those of the formula, bit for bit.
-__device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int half, bool store, uint8_t* codes, uint8_t* scale)
+__device__ __forceinline__ MxBlock mx_swiglu(v16f g, v16f u, float limit, bool exists)
 {
     if (limit > 0.0f) {
 #pragma unroll
@@ -147,7 +163,7 @@ __device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int
     MxScale s = block_scale(__float_as_uint(m));
     // (a block of all but nothing, whose products may have lost bits below the normal numbers, too)
     const bool tiny = s.byte < 32 && m > 0.0f;
-    if (__any(store && (near < (2 * kNear << 11) || least < -32.0f || tiny))) {
+    if (__any(exists && (near < (2 * kNear << 11) || least < -32.0f || tiny))) {
         uint32_t todo = 0;
         // over 2^e a value below 0.1 has the code of zero, even if the block's scale turns out to be half as large
         const float small = 0.1f;
@@ -158,7 +174,7 @@ __device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int
             const bool nothing = s.finite && !tiny && g[i] >= -80.0f && __builtin_fabsf(y[i]) * s.inverse < small;
             if ((key < (2 * kNear << 11) || g[i] < -32.0f || tiny) && g[i] != 0.0f && u[i] != 0.0f && !nothing) todo |= 1u << i;
         }
-        if (!store) todo = 0;
+        if (!exists) todo = 0;
         while (todo) {
             const int at = __builtin_ctz(todo);
             todo &= todo - 1;
@@ -181,33 +197,24 @@ __device__ __forceinline__ void mx_swiglu_store(v16f g, v16f u, float limit, int
     const uint32_t low = s.finite ? mx_codes8(v[0]) : 0, high = s.finite ? mx_codes8(v[1]) : 0;
     // lower half: channels 0-15 of the block, upper half: 16-31
     const v2u p = __builtin_amdgcn_permlane32_swap(low, high, false, false);
-    const uint2 q = make_uint2(__builtin_amdgcn_perm(p[1], p[0], 0x05040100), __builtin_amdgcn_perm(p[1], p[0], 0x07060302));
-    if (store) {
-        *(uint2*)(codes + 8 * half) = q;
-        if (half == 0) *scale = (uint8_t)s.byte;
-    }
+    return {make_uint2(__builtin_amdgcn_perm(p[1], p[0], 0x05040100), __builtin_amdgcn_perm(p[1], p[0], 0x07060302)), s.byte};
 }
 
-// 32 channels of a token as 16-bit values at `to`
+// 16 of 32 channels of a token as 16-bit values: 16 p .. 16 p + 7 in the lower half of the wavefront, + 8 in the upper one
 template <int DT>
-__device__ __forceinline__ void mx_store_half(const v16f& y, int half, bool store, uint16_t* to)
+__device__ __forceinline__ v4u mx_half(const v16f& y, int p)
 {
+    uint32_t d[2][2];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        uint32_t d[2][2];
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int i = 8 * p + 4 * q + 2 * k;
-                d[q][k] = (uint32_t)f32_to_half<DT>(y[i]) | (uint32_t)f32_to_half<DT>(y[i + 1]) << 16;
-            }
-        // lower half: channels 16 p .. + 7, upper half: 16 p + 8 .. + 15
-        const v2u s0 = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
-        const v2u s1 = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
-        const v4u v = {s0[0], s1[0], s0[1], s1[1]};
-        if (store) *(v4u*)(to + 16 * p + 8 * half) = v;
-    }
+        for (int k = 0; k < 2; ++k) {
+            const int i = 8 * p + 4 * q + 2 * k;
+            d[q][k] = (uint32_t)f32_to_half<DT>(y[i]) | (uint32_t)f32_to_half<DT>(y[i + 1]) << 16;
+        }
+    const v2u s0 = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
+    const v2u s1 = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
+    return (v4u){s0[0], s1[0], s0[1], s1[1]};
 }
 
 // (expert, rows) of the 128-row tiles, in the order of the experts

@@ -163,7 +163,7 @@ extern "C" int moe355_gmm_mx(const uint8_t* x, const uint8_t* x_scale, const int
 {
     if (out_dtype != MOE355_DT_BF16 && out_dtype != MOE355_DT_F16) return MOE355_E_ARG;
     const MxArgs a = {x, x_scale, row_token, w, w_scale, group_list, group_list_type, rows, x_rows, k, n, num_experts, 0.0f,
-                      out, nullptr};
+                      out, nullptr, mx_far(rows, n)};
     return run(a, false, out_dtype, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -174,6 +174,6 @@ extern "C" int moe355_gmm_mx_swiglu_quant(const uint8_t* x, const uint8_t* x_sca
                                           size_t workspace_bytes, void* stream)
 {
     const MxArgs a = {x, x_scale, row_token, w, w_scale, group_list, group_list_type, rows, x_rows, k, n, num_experts,
-                      swiglu_limit, out, out_scale};
+                      swiglu_limit, out, out_scale, false};
     return run(a, true, MOE355_DT_BF16, workspace, workspace_bytes, (hipStream_t)stream);
 }

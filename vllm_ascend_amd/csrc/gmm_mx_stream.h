@@ -170,12 +170,19 @@ struct MxStream {
                 }
             }
             if constexpr (EPI == MX_SWIGLU) {
-                mx_swiglu_store(acc[0][t], acc[1][t], a.limit, half, store, (uint8_t*)a.out + row * (a.N / 4) + t0 * 16,
-                                a.out_scale + row * (a.N / 64) + t0);
+                const MxBlock b = mx_swiglu(acc[0][t], acc[1][t], a.limit, store);
+                if (store) {
+                    *(uint2*)((uint8_t*)a.out + row * (a.N / 4) + t0 * 16 + 8 * half) = b.codes;
+                    if (half == 0) a.out_scale[row * (a.N / 64) + t0] = (uint8_t)b.scale;
+                }
             } else {
-                uint16_t* to = (uint16_t*)a.out + row * a.N;
-                mx_store_half<DT>(acc[0][t], half, store, to + t0 * 32);
-                mx_store_half<DT>(acc[1][t], half, row < row1 && store1, to + t1 * 32);
+                uint16_t* to = (uint16_t*)a.out + row * a.N + 8 * half;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const v4u v0 = mx_half<DT>(acc[0][t], p), v1 = mx_half<DT>(acc[1][t], p);
+                    if (store) *(v4u*)(to + t0 * 32 + 16 * p) = v0;
+                    if (row < row1 && store1) *(v4u*)(to + t1 * 32 + 16 * p) = v1;
+                }
             }
         }
     }

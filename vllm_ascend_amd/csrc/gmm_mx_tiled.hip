@@ -101,12 +101,16 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     int64_t row0, row1;
     if (LISTED || !a.group_list) {
         // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one
-        // after the other, so that the tile's tokens and the expert's weights stay in its L2.
+        // after the other, so that the tile's tokens and the expert's weights stay in its L2.  (Every eighth group of 4, 8 or 16
+        // tiles instead, which a workgroup knows without the number of tiles: no faster in listed products, 61 to 180 us instead
+        // of 40 where there are few tiles.)
         const uint32_t count = LISTED ? map.count[0] : (uint32_t)((a.rows + kTileRows - 1) / kTileRows);
         const uint32_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
         if ((blockIdx.x >> 3) >= share || item >= items) return;
-        const int tile = (int)(item / columns);
-        column = (int)(item - tile * columns);
+        // (in bands of 8 columns: the 64 workgroups of an XCD that run at a time share 8 tiles' tokens and 8 columns' weights)
+        const uint32_t band = item / (count * 8), in = item - band * count * 8, wide = min(8u, (uint32_t)columns - band * 8);
+        const int tile = (int)(in / wide);
+        column = (int)(band * 8 + in - tile * wide);
         e = LISTED ? map.expert[tile] : 0;
         row0 = LISTED ? map.begin[tile] : (int64_t)tile * kTileRows;
         row1 = LISTED ? map.end[tile] : a.rows;
@@ -148,13 +152,22 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         const int64_t t = a.row_token[row];
         return t >= 0 && t < a.x_rows ? (uint32_t)t : 0;
     };
+    uint32_t absent = 0;  // bits of this lane's columns of the product whose row is not there
+    if (a.row_token) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int64_t row = row0 + t * 32 + (lane & 31);
+            const int32_t token = a.row_token[row < row1 ? row : row1 - 1];
+            absent |= token < 0 || token >= a.x_rows ? 1u << t : 0;
+        }
+    }
     const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
     uint32_t from[4];
     const int piece = (lane & 7) ^ (lane >> 4);  // of rows 8 i + lane / 8 with even i; with odd ones piece ^ 4
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16;
-    // scales: thread t has row t / 2, half t % 2
+    // scales: thread t has row t / 2, half t % 2 of every window
     const uint32_t scale_from = token_of(row0 + (threadIdx.x >> 1)) * (uint32_t)(a.K / 32);
 
     auto fetch_tokens = [&](int w, int slot) {
@@ -264,32 +277,62 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         window(w, held[0], part);
         held[0] = held[1];
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end still write LDS
     __builtin_amdgcn_s_setprio(0);
-
+    // The results go through LDS, which turns them into whole lines: once the loads past the end have landed and everybody has
+    // read the last window.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const int64_t row = row0 + t * 32 + row_in;
-        const bool store = row < row1 && has0;
-        if (a.row_token) {  // a row that is not there counts as zeros
-            const int64_t token = row < row1 ? a.row_token[row] : 0;
-            const bool there = token >= 0 && token < a.x_rows;
-            if (__any(!there)) {
+        const bool exists = row0 + t * 32 + row_in < row1;
+        if (__any(absent >> t & 1)) {  // a row that is not there counts as zeros
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    acc[0][t][i] = there ? acc[0][t][i] : 0.0f;
-                    acc[1][t][i] = there ? acc[1][t][i] : 0.0f;
-                }
+            for (int i = 0; i < 16; ++i) {
+                acc[0][t][i] = absent >> t & 1 ? 0.0f : acc[0][t][i];
+                acc[1][t][i] = absent >> t & 1 ? 0.0f : acc[1][t][i];
             }
         }
         if constexpr (EPI == MX_SWIGLU) {
-            mx_swiglu_store(acc[0][t], acc[1][t], a.limit, half, store, (uint8_t*)a.out + row * (a.N / 4) + t0 * 16,
-                            a.out_scale + row * (a.N / 64) + t0);
+            // 64 bytes of codes a row, and four scales behind all of them
+            const MxBlock b = mx_swiglu(acc[0][t], acc[1][t], a.limit, exists && has0);
+            *(uint2*)(tokens + (t * 32 + row_in) * 64 + wave * 16 + 8 * half) = b.codes;
+            if (half == 0) tokens[kTileRows * 64 + (t * 32 + row_in) * 4 + wave] = (uint8_t)b.scale;
         } else {
-            uint16_t* to = (uint16_t*)a.out + row * a.N;
-            mx_store_half<DT>(acc[0][t], half, store, to + t0 * 32);
-            mx_store_half<DT>(acc[1][t], half, row < row1 && has1, to + t1 * 32);
+            // 128 bytes a row of this wavefront's 64 channels, the pieces exchanged as the tokens' are; three blocks in turn
+            uint8_t* patch = tokens + (wave * 3 + t % 3) * 4096;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+                    *(v4u*)(patch + row_in * 128 + ((c * 4 + p * 2 + half) ^ (row_in >> 1 & 7)) * 16) = mx_half<DT>(acc[c][t], p);
+            wave_lds_order();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 3), piece = lane & 7;
+                const int64_t row = row0 + t * 32 + r;
+                const v4i v = *(const v4i*)(patch + r * 128 + (piece ^ (r >> 1 & 7)) * 16);
+                if (row < row1 && (piece < 4 ? has0 : has1)) {
+                    if (a.far) __builtin_nontemporal_store(v, (v4i*)((uint16_t*)a.out + row * a.N + b0 * 32 + piece * 8));
+                    else store16_through((uint16_t*)a.out + row * a.N + b0 * 32 + piece * 8, v);
+                }
+            }
+            wave_lds_order();
         }
+    }
+    if constexpr (EPI == MX_SWIGLU) {
+        __syncthreads();
+        // a thread has half of a row
+        const int r = threadIdx.x >> 1, h = threadIdx.x & 1, left = last + 1 - column * 4;  // blocks of 32 channels
+        const int64_t row = row0 + r;
+        if (row >= row1) return;
+        const v4i* from = (const v4i*)(tokens + r * 64 + h * 32);
+        v4i* to = (v4i*)((uint8_t*)a.out + row * (a.N / 4) + column * 64 + h * 32);
+        if (2 * h < left) to[0] = from[0];
+        if (2 * h + 1 < left) to[1] = from[1];
+        uint8_t* scale = a.out_scale + row * (a.N / 64) + column * 4 + h * 2;
+        const uint8_t* held = tokens + kTileRows * 64 + r * 4 + h * 2;
+        if (2 * h < left) scale[0] = held[0];
+        if (2 * h + 1 < left) scale[1] = held[1];
     }
 }
 

@@ -102,9 +102,9 @@ extern "C" int moe355_mx_experts(const void* x, const uint8_t* x_scale, int dtyp
                              b.tiles ? 1 : 0, &built, stream)))
         return rc;
     const MxArgs up = {codes, scale, b.row_token, w13, w13_scale, expert_tokens, MOE355_GL_COUNT, R, T, H, 2 * I, E, swiglu_limit,
-                       b.hidden, b.hidden_scale};
+                       b.hidden, b.hidden_scale, false};
     const MxArgs down = {b.hidden, b.hidden_scale, nullptr, w2, w2_scale, expert_tokens, MOE355_GL_COUNT, R, R, I, H, E, 0.0f, b.out,
-                         nullptr};
+                         nullptr, mx_far(R, H)};
     if (b.tiles && !built) mx_build_map(up, map, st);
     if ((rc = mx_launch(up, true, dtype, b.form13, map, st))) return rc;
     if ((rc = mx_launch(down, false, dtype, b.form2, map, st))) return rc;
