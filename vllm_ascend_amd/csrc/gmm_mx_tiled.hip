@@ -86,7 +86,11 @@ __global__ __launch_bounds__(1024) void mx_map_kernel(const int64_t* __restrict_
     }
 }
 
-template <int EPI, int DT, bool LISTED>
+// GRID: a workgroup has the tile (expert, one of those it may have) of its place in the grid, if there is one; otherwise one of the list, or
+// of the one expert.  (Workgroups that stay and take turns through the list, with the next tile's place and rows known before they
+// are through with one, were slower in every grouped product, 65536 rows of 2048 -> 2 x 768 179 us instead of 160: two that share a
+// compute unit start their tiles together, and what the loop keeps does not fit the registers.)
+template <int EPI, int DT, bool GRID>
 __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxMap map)
 {
     // (not an array of a known size: the compiler would wait for every load on its way to it before each read)
@@ -96,33 +100,29 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int tiles = (int)(a.N / 32), steps = (int)(a.K / 64), windows = (steps + 3) / 4;
     const int columns = EPI == MX_SWIGLU ? (tiles / 2 + 3) / 4 : (tiles + 7) / 8;
-
     int e, column;
     int64_t row0, row1;
-    if (LISTED || !a.group_list) {
-        // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one
-        // after the other, so that the tile's tokens and the expert's weights stay in its L2.  (Every eighth group of 4, 8 or 16
-        // tiles instead, which a workgroup knows without the number of tiles: no faster in listed products, 61 to 180 us instead
-        // of 40 where there are few tiles.)
-        const uint32_t count = LISTED ? map.count[0] : (uint32_t)((a.rows + kTileRows - 1) / kTileRows);
-        const uint32_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
-        if ((blockIdx.x >> 3) >= share || item >= items) return;
-        // (in bands of 8 columns: the 64 workgroups of an XCD that run at a time share 8 tiles' tokens and 8 columns' weights)
-        const uint32_t band = item / (count * 8), in = item - band * count * 8, wide = min(8u, (uint32_t)columns - band * 8);
-        const int tile = (int)(in / wide);
-        column = (int)(band * 8 + in - tile * wide);
-        e = LISTED ? map.expert[tile] : 0;
-        row0 = LISTED ? map.begin[tile] : (int64_t)tile * kTileRows;
-        row1 = LISTED ? map.end[tile] : a.rows;
-    } else {
-        // (column, expert, tile of it): most experts have fewer tiles than they might
-        column = blockIdx.x;
+    if constexpr (GRID) {
         e = blockIdx.y;
+        column = blockIdx.x;
         const int64_t n = a.group_list[e], m = a.gl_type == MOE355_GL_CUMSUM ? n - (e > 0 ? a.group_list[e - 1] : 0) : n;
         if (m <= (int64_t)blockIdx.z * kTileRows) return;
         mx_expert_rows(a, e, lane, row0, row1);
         row0 += (int64_t)blockIdx.z * kTileRows;
         if (row0 >= row1) return;
+    } else {
+        // Consecutive workgroups run on different XCDs; an XCD takes a contiguous part of the tiles, all columns of a tile one
+        // after the other, so that the tile's tokens and the expert's weights stay in its L2, in bands of 8 columns: the 64
+        // workgroups of an XCD that run at a time share 8 tiles' tokens and 8 columns' weights (8192^3 330 -> 268 us).
+        const uint32_t count = map.count ? map.count[0] : (uint32_t)((a.rows + kTileRows - 1) / kTileRows);
+        const uint32_t items = count * columns, share = (items + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= share || item >= items) return;
+        const uint32_t band = item / (count * 8), in = item - band * count * 8, wide = min(8u, (uint32_t)columns - band * 8);
+        const int tile = (int)(in / wide);
+        column = (int)(band * 8 + in - tile * wide);
+        e = map.count ? map.expert[tile] : 0;
+        row0 = map.count ? map.begin[tile] : (int64_t)tile * kTileRows;
+        row1 = map.count ? map.end[tile] : a.rows;
     }
 
     // this wavefront's two blocks of channels (a block past the last one computes the last one again and is not stored)
@@ -145,40 +145,31 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     const auto ws1 = mx_buffer(a.w_scale + ((int64_t)e * tiles + t1) * windows * 256, windows * 256);
 
     // Tokens' bytes of a window: row-major, 128 bytes a row, the 16-byte pieces exchanged by row pair so that the 16 lanes that
-    // LDS serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.
-    auto token_of = [&](int64_t row) -> uint32_t {
-        row = row < row1 ? row : row1 - 1;  // rows behind the last one are not stored
-        if (!a.row_token) return (uint32_t)row;
-        const int64_t t = a.row_token[row];
-        return t >= 0 && t < a.x_rows ? (uint32_t)t : 0;
-    };
-    uint32_t absent = 0;  // bits of this lane's columns of the product whose row is not there
-    if (a.row_token) {
+    // LDS serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.  Scales: thread
+    // t has row t / 2, half t % 2.
+    // (what lies past the end of x reads as zeros: a row that is not there)
+    auto row_of = [&](int64_t row) -> int32_t { return row >= row1 ? -1 : a.row_token ? a.row_token[row] : (int32_t)row; };
+    int32_t token[5];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int64_t row = row0 + t * 32 + (lane & 31);
-            const int32_t token = a.row_token[row < row1 ? row : row1 - 1];
-            absent |= token < 0 || token >= a.x_rows ? 1u << t : 0;
-        }
-    }
+    for (int i = 0; i < 4; ++i) token[i] = row_of(row0 + wave * 32 + i * 8 + (lane >> 3));
+    token[4] = row_of(row0 + (threadIdx.x >> 1));
     const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
+    constexpr uint32_t kNowhere = 0xfff00000;       // past the end of x with any offset into a row (2^19 at most): zeros
+    const auto xb = mx_buffer(a.x, (uint32_t)(a.x_rows * (a.K / 2)));
+    auto there = [&](int32_t t) { return t >= 0 && t < a.x_rows; };
     uint32_t from[4];
     const int piece = (lane & 7) ^ (lane >> 4);  // of rows 8 i + lane / 8 with even i; with odd ones piece ^ 4
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        from[i] = token_of(row0 + wave * 32 + i * 8 + (lane >> 3)) * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16;
-    // scales: thread t has row t / 2, half t % 2 of every window
-    const uint32_t scale_from = token_of(row0 + (threadIdx.x >> 1)) * (uint32_t)(a.K / 32);
+        from[i] = there(token[i]) ? (uint32_t)token[i] * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16 : kNowhere;
+    const uint32_t scale_from = there(token[4]) ? (uint32_t)token[4] * (uint32_t)(a.K / 32) : 0;
 
     auto fetch_tokens = [&](int w, int slot) {
-        // a shorter last window has 32 bytes a step of a row; the pieces behind them are the first one again (not used)
+        // (a shorter last window's last pieces are the next row's, and not used)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = piece ^ (i & 1) * 4;
-            const uint32_t back = w < full || p < 2 * tail ? 0 : p * 16;
-            __builtin_amdgcn_global_load_lds(MOE355_GPTR(a.x + w * 128 + (from[i] - back)),
-                                             MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16, 0, 0);
-        }
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16,
+                                                     from[i] + w * 128, 0, 0, 0);
     };
     const uint32_t scale_end = mx_scale_bytes(a) - 4;
     const auto x_scales = mx_buffer(a.x_scale, scale_end + 4);
@@ -285,13 +276,6 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const bool exists = row0 + t * 32 + row_in < row1;
-        if (__any(absent >> t & 1)) {  // a row that is not there counts as zeros
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                acc[0][t][i] = absent >> t & 1 ? 0.0f : acc[0][t][i];
-                acc[1][t][i] = absent >> t & 1 ? 0.0f : acc[1][t][i];
-            }
-        }
         if constexpr (EPI == MX_SWIGLU) {
             // 64 bytes of codes a row, and four scales behind all of them
             const MxBlock b = mx_swiglu(acc[0][t], acc[1][t], a.limit, exists && has0);
@@ -324,15 +308,16 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         // a thread has half of a row
         const int r = threadIdx.x >> 1, h = threadIdx.x & 1, left = last + 1 - column * 4;  // blocks of 32 channels
         const int64_t row = row0 + r;
-        if (row >= row1) return;
-        const v4i* from = (const v4i*)(tokens + r * 64 + h * 32);
-        v4i* to = (v4i*)((uint8_t*)a.out + row * (a.N / 4) + column * 64 + h * 32);
-        if (2 * h < left) to[0] = from[0];
-        if (2 * h + 1 < left) to[1] = from[1];
-        uint8_t* scale = a.out_scale + row * (a.N / 64) + column * 4 + h * 2;
-        const uint8_t* held = tokens + kTileRows * 64 + r * 4 + h * 2;
-        if (2 * h < left) scale[0] = held[0];
-        if (2 * h + 1 < left) scale[1] = held[1];
+        if (row < row1) {
+            const v4i* held = (const v4i*)(tokens + r * 64 + h * 32);
+            v4i* to = (v4i*)((uint8_t*)a.out + row * (a.N / 4) + column * 64 + h * 32);
+            if (2 * h < left) to[0] = held[0];
+            if (2 * h + 1 < left) to[1] = held[1];
+            uint8_t* scale = a.out_scale + row * (a.N / 64) + column * 4 + h * 2;
+            const uint8_t* held_scale = tokens + kTileRows * 64 + r * 4 + h * 2;
+            if (2 * h < left) scale[0] = held_scale[0];
+            if (2 * h + 1 < left) scale[1] = held_scale[1];
+        }
     }
 }
 
@@ -359,13 +344,13 @@ void mx_build_map(const MxArgs& a, const MxMap& map, hipStream_t st)
 int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, const MxMap& map, hipStream_t st)
 {
     const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, tiles = (a.rows + kTileRows - 1) / kTileRows;
-    const int64_t most = form == MX_LISTED ? mx_most_tiles(a.rows, a.E) : tiles, groups = (most * columns + 7) / 8 * 8;
-    if (groups > 0x7fffffff) return MOE355_E_SHAPE;
     const bool direct = form == MX_TILES && a.group_list;
+    const int64_t most = (form == MX_LISTED ? mx_most_tiles(a.rows, a.E) : tiles) * columns, groups = (most + 7) / 8 * 8;
+    if (most > 0x7fffffff) return MOE355_E_SHAPE;
     const dim3 grid = direct ? dim3((unsigned)columns, (unsigned)a.E, (unsigned)tiles) : dim3((unsigned)groups);
 #define MOE355_MXT(E_, D_)                                                                                       \
     do {                                                                                                         \
-        if (form == MX_LISTED)                                                                                   \
+        if (direct)                                                                                              \
             hipLaunchKernelGGL((gmm_mx_tiled_kernel<E_, D_, true>), grid, dim3(kThreads), kLds, st, a, map);     \
         else                                                                                                     \
             hipLaunchKernelGGL((gmm_mx_tiled_kernel<E_, D_, false>), grid, dim3(kThreads), kLds, st, a, map);    \
