@@ -580,7 +580,7 @@ int moe355_layer_gates_inside(const moe355_layer *layer /* host */, int64_t num_
  * max(floor(log2 a) - 2, -127) (a = 0: -127), codes rounded to nearest even, magnitudes above 6 to 6; a block with an
  * infinity or NaN: scale byte 255, which stands for NaN, codes 0.
  * Stand in for torch_npu.npu_dynamic_mx_quant and its inverse (the MXFP4 branch of vllm_ascend/device/device_op.py:192-206).
- * cols % 32 == 0 and at most 2^20; x, out 16-byte and codes 4-byte aligned (MOE355_E_SHAPE otherwise).
+ * cols % 32 == 0 and at most 2^20, rows * cols below 2^35; x, out 16-byte and codes 4-byte aligned (MOE355_E_SHAPE otherwise).
  * x [rows, cols] fp32 / bf16 / fp16 -> codes [rows, cols / 2], scale [rows, cols / 32]; and back. */
 int moe355_dynamic_mx_quant(const void *x, int x_dtype, int64_t rows, int64_t cols, uint8_t *codes, uint8_t *scale,
                             void *stream);
@@ -593,14 +593,15 @@ int moe355_mx_dequant(const uint8_t *codes, const uint8_t *scale, int64_t rows, 
  *   (MOE355_NORM_MXFP4) make of y; MOE355_NORM_PLAIN: y alone.
  * x1, x2, x, y [rows, cols] of x_dtype (bf16 / fp16); gamma, beta [cols] of weight_dtype (x_dtype or fp32), beta may be
  * NULL.  x and y may be NULL (not wanted; MOE355_NORM_PLAIN needs y); x may be the same buffer as x1 or x2.
- * cols % 8 == 0 (MXFP4: 32) and at most 2^20; rows and weights 16-byte aligned. */
+ * cols % 8 == 0 (MXFP4: 32) and at most 2^20; rows below 2^22 (2^26 of up to 512 values, the limit in between: a launch has
+ * 2^32 threads); rows and weights 16-byte aligned. */
 enum { MOE355_NORM_PLAIN = 0, MOE355_NORM_INT8 = 1, MOE355_NORM_MXFP4 = 2 };
 int moe355_add_rms_norm_quant(const void *x1, const void *x2, const void *gamma, const void *beta, int x_dtype,
                               int weight_dtype, int64_t rows, int64_t cols, double epsilon, int kind, void *x, void *y,
                               void *q, void *scale, void *stream);
 
 /* Weights [E, n, k / 2] codes and [E, n, k / 32] scales to the storage of the products below: as many bytes of codes, and
- * E * n * ceil(k / 256) * 8 bytes of scales.  n % 32 == 0, k % 64 == 0. */
+ * E * n * ceil(k / 256) * 8 bytes of scales.  n % 32 == 0, k % 64 == 0, E * n * k below 2^37. */
 int moe355_format_cast_mx(const uint8_t *codes, const uint8_t *scale, int64_t num_experts, int64_t n, int64_t k,
                           uint8_t *codes_out, uint8_t *scale_out, void *stream);
 

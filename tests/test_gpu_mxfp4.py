@@ -405,9 +405,12 @@ def experts_ref(y, ids, weights, w13, w2, dtype, residual=None):
 
 def close(got, want, dtype, k):
     """One rounding to 16 bits (half a step) and k additions in 32 bits: 2^-8 or 2^-11 of the value plus k 2^-24 of the terms'
-    size, for which the row's largest value times sqrt(k) stands."""
+    size, for which the row's largest value times sqrt(k) stands.  Below the smallest normal number 2^m the type's steps are all
+    2^m eps (fp16: 2^-14 2^-10 = 2^-24), so the rounding there is off by up to 2^m eps / 2 however small the value."""
     got = got.double().cpu().numpy()
-    bound = np.abs(want) * torch.finfo(dtype).eps / 2 * 1.001 + k * 2.0 ** -24 * np.abs(want).max(-1, keepdims=True) * 4
+    info = torch.finfo(dtype)
+    bound = np.maximum(np.abs(want), info.smallest_normal) * info.eps / 2 * 1.001
+    bound += k * 2.0 ** -24 * np.abs(want).max(-1, keepdims=True) * 4
     return bool((np.abs(got - want) <= bound).all())
 
 
@@ -533,3 +536,203 @@ def test_layer_of_no_tokens(ops):
     out = layer.quant_method.apply(layer, torch.empty(0, 512, dtype=torch.bfloat16, device=DEV),
                                    torch.empty(0, 2, device=DEV), torch.empty(0, 2, dtype=torch.int32, device=DEV)).routed_out
     assert out.shape == (0, 512)
+
+
+# ------------------------------------------------------------------------------------------------ where it can go wrong
+def both_products(K, E, N, Kd, x, x_scale, w, s, gl, list_type=1, row_map=None):
+    """-> (16-bit rows, codes, scales) of the two forms of output."""
+    return (K.gmm_mx(x, x_scale, w, s, gl, list_type, row_map=row_map),
+            *K.gmm_mx_swiglu_quant(x, x_scale, w, s, gl, list_type, row_map=row_map))
+
+
+def check_both(got, acc, used=None):
+    out, codes, scale = (t[:used] for t in got)
+    acc = acc[:used]
+    with np.errstate(invalid="ignore"):
+        want = ref.rounded(acc, out.dtype)
+        c, sc = ref.quantise(ref.swiglu(acc))
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(out.cpu()), nan)
+    assert same_bits(out.cpu().masked_fill(nan, 0), want.masked_fill(nan, 0))
+    assert np.array_equal(scale.cpu().numpy(), sc) and np.array_equal(codes.cpu().numpy(), ref.pack(c))
+
+
+@pytest.mark.parametrize("rows", [9, 600])
+def test_rows_that_are_not_there_have_nobodys_scale(K, rows):
+    """Row 0 of x has no value (its scales stand for NaN), and a block of weights has none either: a row that is not there is
+    zeros times the weights, NaN in that block's channel only."""
+    say("absent rows beside NaN", rows)
+    E, N, Kd, tokens = 2, 128, 320, 5
+    _, counts, row_token, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even", tokens=tokens)
+    xs[0] = 255
+    ws[1, 3, 2] = 255
+    row_token[row_token == 0] = 1
+    row_token[::3] = -1
+    row_token[1::5] = tokens
+    row_token[2::7] = 0
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    got = both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, dev(counts.astype(np.int64)), row_map=dev(row_token))
+    with np.errstate(invalid="ignore"):
+        check_both(got, ref.products(ref.values(xc, xs), ref.values(wc, ws), counts, row_token))
+
+
+@pytest.mark.parametrize("E,rows,kind", [(600, 4000, "zipf"), (1100, 4500, "even"), (600, 3700, "one")])
+@pytest.mark.parametrize("list_type", [0, 1])
+def test_tiles_from_a_list(K, E, rows, kind, list_type):
+    """Many experts with many rows each could have: the products make a list of the tiles first."""
+    from vllm_ascend_amd import _lib
+
+    say("listed tiles", E, rows, kind, list_type)
+    N, Kd = 64, 128
+    assert _lib.load().moe355_gmm_mx_workspace(rows, N, E, 0) and _lib.load().moe355_gmm_mx_workspace(rows, N, E, 1)
+    _, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, kind)
+    counts[0] = max(counts[0] - 5, 0)  # rows behind the last group
+    used = int(counts.sum())
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    gl = dev(np.asarray(counts if list_type else counts.cumsum()).astype(np.int64))
+    x, x_scale = dev(ref.pack(xc)), dev(xs)
+    acc = ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)
+    check_both(both_products(K, E, N, Kd, x, x_scale, w, s, gl, list_type), acc, used)
+    check_both(both_products(K, E, N, Kd, x, x_scale, w, s, gl.int(), list_type), acc, used)
+
+
+@pytest.mark.parametrize("list_type", [0, 1])
+def test_lists_of_tiles_out_of_range(K, list_type):
+    say("listed tiles, lists out of range", list_type)
+    E, N, Kd, rows = 600, 64, 64, 4000
+    _, _, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    counts = np.zeros(E, dtype=np.int64)
+    counts[[0, 2, 599]] = [1500, 1, 2499]
+    gl = np.zeros(E, dtype=np.int64)
+    if list_type:
+        gl[0], gl[1], gl[2], gl[599] = 1500, -7, 1, 1 << 45
+    else:
+        gl[:2], gl[2:599], gl[599] = 1500, 1501, 1 << 45
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    got = both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, dev(gl), list_type)
+    check_both(got, ref.products(ref.values(xc, xs), ref.values(wc, ws), counts))
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_operands_that_are_views(K, rows):
+    """Scales at odd addresses, codes that no wide load may start at, transposed and strided operands, lists of int32."""
+    say("views", rows)
+    E, N, Kd = 2, 128, 192
+    _, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    x, x_scale = dev(ref.pack(xc)), dev(xs)
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    acc = ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)
+
+    def at(t, offset):
+        room = torch.zeros(t.numel() + offset, dtype=torch.uint8, device=DEV)
+        room[offset:] = t.flatten()
+        return room[offset:].view(t.shape)
+
+    gl = dev(counts.astype(np.int32))
+    check_both(both_products(K, E, N, Kd, at(x, 8), at(x_scale, 1), at(w, 4), at(s, 3), gl), acc)
+    check_both(both_products(K, E, N, Kd, x.t().contiguous().t(), x_scale.t().contiguous().t(), w, s, gl), acc)
+    check_both(both_products(K, E, N, Kd, x.repeat_interleave(2, 0)[::2], x_scale.repeat(1, 2)[:, :Kd // 32], w, s, gl), acc)
+    w2, s2 = K.format_cast_mx(at(dev(ref.pack(wc)), 8), at(dev(ws), 1))
+    assert torch.equal(w2, w) and torch.equal(s2, s)
+
+
+def test_one_row_with_two_scales(ops):
+    """K = 64: less memory at the scales than the kernels read at a time."""
+    say("two scales")
+    _, _, _, xc, xs, wc, ws = make_product(1, 32, 64, 1, "even")
+    w, s = ops.npu_format_cast_mx(dev(ref.pack(wc[0])), dev(ws[0]))
+    out = ops.npu_quant_matmul(dev(ref.pack(xc)), w, s, pertoken_scale=dev(xs), output_dtype=torch.bfloat16)
+    assert same_bits(out, ref.rounded(ref.values(xc, xs) @ ref.values(wc, ws)[0].T, torch.bfloat16))
+
+
+def test_output_larger_than_the_last_cache(K):
+    """Such an output is stored past it; channels repeat, so that the reference stays small."""
+    say("far stores")
+    rows, Kd, distinct, times = 3210, 64, 1024, 32
+    _, _, _, xc, xs, wc, ws = make_product(1, distinct, Kd, rows, "even")
+    w, s = K.format_cast_mx(dev(ref.pack(wc)).repeat(1, times, 1), dev(ws).repeat(1, times, 1))
+    out = K.gmm_mx(dev(ref.pack(xc)), dev(xs), w, s, None, 1)
+    want = ref.rounded(ref.values(xc, xs) @ ref.values(wc, ws)[0].T, torch.bfloat16).to(DEV)
+    for part in out.view(rows, times, distinct).unbind(1):
+        assert torch.equal(part, want)
+
+
+def op_by_op(K, x, x_scale, ids, weights, w13, s13, w2, s2, limit, residual):
+    if x_scale is None:
+        x, x_scale = K.dynamic_mx_quant(x)
+    dst, row_token, tokens = K.route_map(ids, w13.shape[0], 1)
+    h, hs = K.gmm_mx_swiglu_quant(x, x_scale, w13, s13, tokens, 1, limit, row_token)
+    out = K.gmm_mx(h, hs, w2, s2, tokens, 1, weights.dtype)
+    return K.token_unpermute(out, dst, weights, residual), tokens
+
+
+@pytest.mark.parametrize("T,E,k,H,I,dtype", [
+    (1, 8, 2, 64, 64, torch.bfloat16), (40, 16, 4, 320, 192, torch.float16), (900, 8, 2, 256, 448, torch.bfloat16),
+    (2100, 600, 2, 64, 64, torch.bfloat16),   # listed tiles, more experts than one launch of the routing has
+    (1200, 400, 5, 64, 64, torch.float16),    # listed tiles, their list made by the routing
+    (9000, 16, 8, 128, 64, torch.bfloat16)])  # more rows than one launch of the routing has
+def test_experts_as_one_call(K, T, E, k, H, I, dtype):
+    """The same bits as the operators one after the other; ids outside the experts count for nothing."""
+    say("experts", T, E, k, H, I, dtype)
+    rng = np.random.default_rng(T)
+    w13, s13 = ref.random_mx(rng, (E, 2 * I, H), 1)
+    w2, s2 = ref.random_mx(rng, (E, H, I), 1)
+    held = (*K.format_cast_mx(dev(ref.pack(w13)), dev(s13 - 5)), *K.format_cast_mx(dev(ref.pack(w2)), dev(s2 - 5)))
+    g = torch.Generator().manual_seed(T)
+    x, residual = (torch.randn(T, H, generator=g).to(dtype).to(DEV) for _ in range(2))
+    weights = torch.rand(T, k, generator=g).to(dtype).to(DEV)
+    ids = torch.from_numpy((rng.zipf(1.3, (T, k)) % E).astype(np.int32)).to(DEV)
+    outside = ids.clone()
+    outside.view(-1)[::3] = -1
+    outside.view(-1)[1::7] = E
+    for chosen in (ids, outside):
+        for limit, res in ((0.0, None), (0.5, residual)):
+            want, want_tokens = op_by_op(K, x, None, chosen, weights, *held, limit, res)
+            for given in ((x, None), K.dynamic_mx_quant(x)):
+                out, tokens = K.mx_experts(*given, chosen, weights, *held, limit, res)
+                assert torch.equal(tokens, want_tokens) and torch.equal(out, want)
+    nothing, none = K.mx_experts(x, None, torch.full_like(ids, -1), weights, *held)
+    assert not nothing.any() and not none.any()
+    # the rows whose ids are all inside, against the formula
+    y = experts_ref(x[:64], ids[:64].cpu().numpy(), weights[:64], ref.values(w13, s13 - 5), ref.values(w2, s2 - 5), dtype)
+    assert close(K.mx_experts(x, None, ids, weights, *held)[0][:64], y, dtype, k)
+
+
+def test_layer_of_rows_in_three_dimensions(ops):
+    say("three dimensions")
+    layer, _, _ = build(8, 2, 512, 256)
+    g = torch.Generator().manual_seed(6)
+    x, logits = torch.randn(30, 512, generator=g).to(torch.bfloat16).to(DEV), torch.randn(30, 8, generator=g).to(DEV)
+    weights, ids = layer.router.select_experts(x, logits)
+    want = layer.quant_method.apply(layer, x, weights, ids).routed_out
+    assert torch.equal(layer.quant_method.apply(layer, x.view(3, 10, 512), weights, ids).routed_out, want.view(3, 10, 512))
+    codes, layer.ascend_pertoken_scale = (t.view(3, 10, -1) for t in ops.npu_dynamic_mx_quant(x))
+    assert torch.equal(layer.quant_method.apply(layer, codes, weights, ids).routed_out, want.view(3, 10, 512))
+
+
+def test_products_captured_and_replayed_on_two_streams(K):
+    """Two graphs of the same product, one of listed tiles, replayed on two streams at once on changing rows."""
+    say("products in graphs")
+    E, N, Kd, rows = 600, 64, 128, 4000
+    _, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "zipf")
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    x, x_scale, gl = dev(ref.pack(xc)), dev(xs), dev(counts.astype(np.int64))
+    both_products(K, E, N, Kd, x, x_scale, w, s, gl)
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for _ in streams:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both_products(K, E, N, Kd, x, x_scale, w, s, gl)
+        graphs.append((graph, out))
+    for i in range(4):
+        x.copy_(torch.roll(x, 1, 0))
+        gl.copy_(torch.roll(gl, 7, 0))
+        want = both_products(K, E, N, Kd, x, x_scale, w, s, gl)
+        torch.cuda.synchronize()
+        for stream, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))

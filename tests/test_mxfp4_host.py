@@ -227,3 +227,41 @@ def test_checkpoint_tensors_under_the_names_of_their_types():
     raw = {n: torch.randint(0, 255, p.shape, generator=g, dtype=torch.uint8) for n, p in layer.named_parameters()}
     layer.load_weights({n: t.view(torch.float8_e8m0fnu if n.endswith("scale") else FP4) for n, t in raw.items()})
     assert all(torch.equal(getattr(layer, n), t) for n, t in raw.items())
+
+
+def test_checkpoint_loader_keeps_the_bytes():
+    from vllm_ascend_amd.quantization.checkpoint import moe_weight_loader
+
+    g = torch.Generator().manual_seed(1)
+    codes, scale = torch.randint(0, 256, (64, 32), generator=g, dtype=torch.uint8), torch.randint(0, 255, (64, 2), generator=g, dtype=torch.uint8)
+    w, s = (torch.nn.Parameter(torch.zeros(2, 128, n, dtype=torch.uint8), requires_grad=False) for n in (32, 2))
+    for c, sc in ((codes, scale), (codes.view(FP4), scale.view(torch.float8_e8m0fnu))):
+        w.data.zero_(), s.data.zero_()
+        moe_weight_loader(w, c, "w13_weight", "w3", 1)
+        moe_weight_loader(s, sc, "w13_weight_scale", "w3", 1)
+        assert torch.equal(w[1, 64:], codes) and torch.equal(s[1, 64:], scale) and not w[0].any() and not w[1, :64].any()
+
+
+def test_experts_refuse(lib):
+    def call(x=P, xs=None, dt=1, T=4, H=128, ids=P, tw=P, k=2, w13=P, s13=P, w2=P, s2=P, I=64, E=8, res=None, tokens=P, out=P, ws=P,
+             less=0):
+        space = lib.moe355_mx_experts_workspace(T, k, H, I, E, int(xs is not None))
+        return lib.moe355_mx_experts(x, xs, dt, T, H, ids, tw, k, w13, s13, w2, s2, I, E, 0.0, res, tokens, out, ws, space - less, None)
+
+    assert call(T=0) == 0
+    for bad in (dict(x=None), dict(ids=None), dict(tw=None), dict(w13=None), dict(s13=None), dict(w2=None), dict(s2=None),
+                dict(tokens=None), dict(out=None), dict(dt=0), dict(T=-1), dict(k=0), dict(H=0), dict(I=0), dict(E=0)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(H=96), dict(I=96), dict(k=65), dict(E=2049), dict(T=1 << 30), dict(x=P + 8), dict(w13=P + 8), dict(s13=P + 2),
+                dict(w2=P + 8), dict(s2=P + 1), dict(out=P + 8), dict(res=P + 8), dict(H=(1 << 20) + 64), dict(I=(1 << 19) + 64)):
+        assert call(**bad) == -2, bad
+    assert call(ws=None) == -3 and call(ws=P + 16) == -3 and call(less=1) == -3
+
+
+def test_launches_larger_than_there_are(lib):
+    """More threads than a launch has."""
+    assert lib.moe355_dynamic_mx_quant(P, 1, 1 << 15, 1 << 20, P, P, None) == -2
+    assert lib.moe355_mx_dequant(P, P, 1 << 15, 1 << 20, P, 1, None) == -2
+    norm = lambda rows, cols: lib.moe355_add_rms_norm_quant(P, P, P, None, 1, 1, rows, cols, 1e-6, 1, P, P, P, P, None)
+    assert norm(1 << 26, 512) == -2 and norm(1 << 22, 16384) == -2
+    assert lib.moe355_format_cast_mx(P, P, 32768, 1 << 16, 64, P, P, None) == -2

@@ -68,6 +68,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint3
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
 }
 
+// A row that is not there has this offset: past the end of x, and of its scales, with any offset into a row added (2^19 at most),
+// so zeros times 2^-127.
+constexpr uint32_t kMxNowhere = 0xfff00000;
+
 __device__ __forceinline__ uint32_t mx_scale_bytes(const MxArgs& a)
 {
     const int64_t n = a.x_rows * (a.K / 32);

@@ -22,8 +22,8 @@ __global__ __launch_bounds__(256) void mx_format_kernel(const uint8_t* __restric
 }
 
 // Few rows an expert: a workgroup has 64 channels of an expert and its rows, 32 at a time (every gridDim.z-th 32); its wavefronts
-// have a part of K each and add their sums through LDS.  Three workgroups' wavefronts a SIMD (168 registers), which is why the form of 64 rows is not
-// here.
+// have a part of K each and add their sums through LDS.  Three wavefronts a SIMD (168 registers), which is why the form of 64 rows
+// is not here.
 template <int EPI, int DT>
 __global__ __launch_bounds__(512, 3) void gmm_mx_stream_kernel(MxArgs a)
 {
@@ -80,7 +80,7 @@ int mx_check(const MxArgs& a, bool swiglu)
     if (a.K % 64 || a.N % (swiglu ? 64 : 32) || a.K > (int64_t)1 << 20 || a.N > (int64_t)1 << 20 || a.E > 32768)
         return MOE355_E_SHAPE;
     // rows of x are reached by offsets of 32 bits
-    if (a.rows > 0x7fffffff || a.x_rows > 0x7fffffff || a.x_rows * (a.K / 2) > 0xfff00000) return MOE355_E_SHAPE;
+    if (a.rows > 0x7fffffff || a.x_rows > 0x7fffffff || a.x_rows * (a.K / 2) > kMxNowhere) return MOE355_E_SHAPE;
     if (a.rows == 0) return MOE355_OK;
     if (a.x_rows == 0 || !a.x || !a.x_scale || !a.w || !a.w_scale || (!a.group_list && a.E > 1) || !a.out || (swiglu && !a.out_scale))
         return MOE355_E_ARG;
@@ -144,7 +144,7 @@ extern "C" int moe355_format_cast_mx(const uint8_t* codes, const uint8_t* scale,
     if (!codes || !scale || !codes_out || !scale_out) return MOE355_E_ARG;
     if (!aligned(codes, 16) || !aligned(codes_out, 16)) return MOE355_E_SHAPE;
     const int64_t channels = num_experts * n, groups = (channels / 32 * (k / 64) * 64 + 255) / 256;
-    if (groups > 0x7fffffff) return MOE355_E_SHAPE;
+    if (groups > 0xffffffff / 256) return MOE355_E_SHAPE;  // a launch has at most 2^32 - 1 threads
     hipLaunchKernelGGL(mx_format_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes, scale, channels, k,
                        codes_out, scale_out);
     return launch_status();

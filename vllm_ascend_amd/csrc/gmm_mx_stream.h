@@ -62,11 +62,12 @@ struct MxStream {
     }
 
     template <int MT, bool WHOLE>
-    __device__ __forceinline__ void multiply(const Weights& w, const Tokens<MT>& x, int nb, v16f (&acc)[2][MT]) const
+    __device__ __forceinline__ void multiply(const Weights& w, const Tokens<MT>& x, const bool (&there)[MT], int nb,
+                                             v16f (&acc)[2][MT]) const
     {
         int s[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) s[t] = x.s[t].get();
+        for (int t = 0; t < MT; ++t) s[t] = there[t] ? x.s[t].get() : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (WHOLE || j < nb) {
@@ -78,7 +79,6 @@ struct MxStream {
             }
     }
 
-    // rows r .. r + 32 MT - 1 of those up to row1
     __device__ __forceinline__ void operands(int e)
     {
         const int64_t tiles = a.N / 32, steps = a.K / 64, windows = (steps + 3) / 4, b0 = e * tiles + t0, b1 = e * tiles + t1;
@@ -93,6 +93,7 @@ struct MxStream {
         xsb = mx_buffer(a.x_scale, scale_end + 4);
     }
 
+    // rows r .. r + 32 MT - 1 of those up to row1; ONCE: nobody else reads these weights
     template <int MT, bool ONCE>
     __device__ __forceinline__ void rows(int64_t r, int64_t row1)
     {
@@ -104,11 +105,10 @@ struct MxStream {
         for (int t = 0; t < MT; ++t) {
             int64_t row = r + t * 32 + (lane & 31);
             row = row < row1 ? row : row1 - 1;  // not stored
-            int64_t token = a.row_token ? a.row_token[row] : row;
+            const int64_t token = a.row_token ? a.row_token[row] : row;
             there[t] = token >= 0 && token < a.x_rows;
-            if (!there[t]) token = 0;
-            x[t] = (uint32_t)token * (uint32_t)(a.K / 2);
-            xs[t] = (uint32_t)token * (uint32_t)(a.K / 32);
+            x[t] = there[t] ? (uint32_t)token * (uint32_t)(a.K / 2) : kMxNowhere;
+            xs[t] = there[t] ? (uint32_t)token * (uint32_t)(a.K / 32) : 0;
         }
         v16f acc[2][MT] = {};
         if (w_begin < w_end) {
@@ -120,18 +120,18 @@ struct MxStream {
                 fetch_weights<ONCE>(w + 1, held[1]);
                 fetch_tokens<MT>(w + 1, x, xs, tokens[1]);
                 __builtin_amdgcn_sched_barrier(0);
-                multiply<MT, true>(held[0], tokens[0], 4, acc);
+                multiply<MT, true>(held[0], tokens[0], there, 4, acc);
                 __builtin_amdgcn_sched_barrier(0);
                 fetch_weights<ONCE>(w + 2, held[0]);
                 fetch_tokens<MT>(w + 2, x, xs, tokens[0]);
                 __builtin_amdgcn_sched_barrier(0);
-                multiply<MT, true>(held[1], tokens[1], 4, acc);
+                multiply<MT, true>(held[1], tokens[1], there, 4, acc);
                 __builtin_amdgcn_sched_barrier(0);
             }
             for (; w < w_end; ++w) {  // at most two more, of which the last one may be short
                 fetch_weights<ONCE>(w + 1, held[1]);
                 fetch_tokens<MT>(w + 1, x, xs, tokens[1]);
-                multiply<MT, false>(held[0], tokens[0], w < full ? 4 : tail, acc);
+                multiply<MT, false>(held[0], tokens[0], there, w < full ? 4 : tail, acc);
                 held[0] = held[1];
                 tokens[0] = tokens[1];
             }
@@ -162,13 +162,6 @@ struct MxStream {
             if (t % waves != wave) continue;
             const int64_t row = r + t * 32 + (lane & 31);
             const bool store = row < row1 && store0;
-            if (__any(!there[t])) {  // a row that is not there counts as zeros
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    acc[0][t][i] = there[t] ? acc[0][t][i] : 0.0f;
-                    acc[1][t][i] = there[t] ? acc[1][t][i] : 0.0f;
-                }
-            }
             if constexpr (EPI == MX_SWIGLU) {
                 const MxBlock b = mx_swiglu(acc[0][t], acc[1][t], a.limit, store);
                 if (store) {

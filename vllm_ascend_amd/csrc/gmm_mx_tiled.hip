@@ -18,7 +18,6 @@ constexpr int kRing = 3;
 constexpr int kStage = kTileRows * 128;  // tokens' bytes of a window
 constexpr int kLds = kRing * (kStage + kTileRows * 8);
 
-#define MOE355_GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define MOE355_LPTR(p) ((__attribute__((address_space(3))) void*)(p))
 
 // One workgroup; thread t has the experts [t seg, (t + 1) seg).  Rows are cut to those that exist.
@@ -147,22 +146,20 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     // Tokens' bytes of a window: row-major, 128 bytes a row, the 16-byte pieces exchanged by row pair so that the 16 lanes that
     // LDS serves at a time find theirs in different banks.  A load fills 8 rows; wavefront v has rows 32 v .. + 31.  Scales: thread
     // t has row t / 2, half t % 2.
-    // (what lies past the end of x reads as zeros: a row that is not there)
     auto row_of = [&](int64_t row) -> int32_t { return row >= row1 ? -1 : a.row_token ? a.row_token[row] : (int32_t)row; };
     int32_t token[5];
 #pragma unroll
     for (int i = 0; i < 4; ++i) token[i] = row_of(row0 + wave * 32 + i * 8 + (lane >> 3));
     token[4] = row_of(row0 + (threadIdx.x >> 1));
     const int tail = steps & 3, full = steps >> 2;  // steps of a last, shorter window; whole windows
-    constexpr uint32_t kNowhere = 0xfff00000;       // past the end of x with any offset into a row (2^19 at most): zeros
     const auto xb = mx_buffer(a.x, (uint32_t)(a.x_rows * (a.K / 2)));
     auto there = [&](int32_t t) { return t >= 0 && t < a.x_rows; };
     uint32_t from[4];
     const int piece = (lane & 7) ^ (lane >> 4);  // of rows 8 i + lane / 8 with even i; with odd ones piece ^ 4
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        from[i] = there(token[i]) ? (uint32_t)token[i] * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16 : kNowhere;
-    const uint32_t scale_from = there(token[4]) ? (uint32_t)token[4] * (uint32_t)(a.K / 32) : 0;
+        from[i] = there(token[i]) ? (uint32_t)token[i] * (uint32_t)(a.K / 2) + (piece ^ (i & 1) * 4) * 16 : kMxNowhere;
+    const uint32_t scale_from = there(token[4]) ? (uint32_t)token[4] * (uint32_t)(a.K / 32) : kMxNowhere;
 
     auto fetch_tokens = [&](int w, int slot) {
         // (a shorter last window's last pieces are the next row's, and not used)
@@ -171,8 +168,8 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
             __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, MOE355_LPTR(tokens + slot * kStage + (wave * 4 + i) * 1024), 16,
                                                      from[i] + w * 128, 0, 0, 0);
     };
-    const uint32_t scale_end = mx_scale_bytes(a) - 4;
-    const auto x_scales = mx_buffer(a.x_scale, scale_end + 4);
+    const auto x_scales = mx_buffer(a.x_scale, mx_scale_bytes(a));
+    const uint32_t scale_end = scale_from == kMxNowhere ? 0xffffffff : mx_scale_bytes(a) - 4;
     auto fetch_scale = [&](int w) {
         MxRowScales s;
         s.fetch(x_scales, scale_from + w * 8 + (threadIdx.x & 1) * (w < full ? 4 : tail), scale_end);
@@ -346,7 +343,7 @@ int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, co
     const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, tiles = (a.rows + kTileRows - 1) / kTileRows;
     const bool direct = form == MX_TILES && a.group_list;
     const int64_t most = (form == MX_LISTED ? mx_most_tiles(a.rows, a.E) : tiles) * columns, groups = (most + 7) / 8 * 8;
-    if (most > 0x7fffffff) return MOE355_E_SHAPE;
+    if (groups > 0xffffffff / kThreads) return MOE355_E_SHAPE;  // a launch has at most 2^32 - 1 threads
     const dim3 grid = direct ? dim3((unsigned)columns, (unsigned)a.E, (unsigned)tiles) : dim3((unsigned)groups);
 #define MOE355_MXT(E_, D_)                                                                                       \
     do {                                                                                                         \

@@ -48,7 +48,7 @@ bool bad_sizes(int64_t T, int k, int64_t H, int64_t I, int E)
 bool unsupported(int64_t T, int k, int64_t H, int64_t I, int E)
 {
     return H % 64 || I % 64 || H > (int64_t)1 << 20 || I > (int64_t)1 << 19 || k > 64 || E > 2048 || T > 0x7ffffffe / k ||
-           T * (H / 2) > 0xfff00000 || T * k * (I / 2) > 0xfff00000;
+           T * (H / 2) > kMxNowhere || T * k * (I / 2) > kMxNowhere;
 }
 
 }  // namespace

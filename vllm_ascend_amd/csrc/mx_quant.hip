@@ -7,6 +7,7 @@ namespace moe355 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMostThreads = 0xffffffff;  // of a launch
 
 // Eight values a thread, a block of 32 by four neighbouring lanes.  HBM bound: 2 (4) bytes in and 17/32 out a value.
 template <int DT>
@@ -254,16 +255,30 @@ __global__ __launch_bounds__(1024) void norm_quant_kernel(NormArgs a)
     }
 }
 
-template <int DT, int GDT, int KIND>
-void launch_norm(const NormArgs& a, int64_t rows, hipStream_t st)
+// Pieces of eight values a thread (0: as many as it takes) and threads a row
+struct NormShape {
+    int per_thread;
+    unsigned threads;
+};
+NormShape norm_shape(int64_t cols)
 {
-    const int64_t nv = a.cols >> 3;
+    const int64_t nv = cols >> 3;
     const unsigned waves = (unsigned)((nv + 63) / 64);
     // Two pieces a thread from 512 on: 4096 rows of 7168 to int8 74.1 -> 65.9 us, to MXFP4 59.6 -> 56.6 (four 65.7, 56.5, but a row
     // alone 7.7 instead of 6.3); 8192 rows of 2048 33.4 with one, 35.8 with two.
-    if (nv <= 512) hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 1>), dim3((unsigned)rows), dim3(64 * waves), 0, st, a);
-    else if (nv <= 2048) hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 2>), dim3((unsigned)rows), dim3(64 * ((waves + 1) / 2)), 0, st, a);
-    else hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 0>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+    if (nv <= 512) return {1, 64 * waves};
+    if (nv <= 2048) return {2, 64 * ((waves + 1) / 2)};
+    return {0, 1024};
+}
+
+template <int DT, int GDT, int KIND>
+void launch_norm(const NormArgs& a, int64_t rows, hipStream_t st)
+{
+    const NormShape s = norm_shape(a.cols);
+    const dim3 grid((unsigned)rows), threads(s.threads);
+    if (s.per_thread == 1) hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 1>), grid, threads, 0, st, a);
+    else if (s.per_thread == 2) hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 2>), grid, threads, 0, st, a);
+    else hipLaunchKernelGGL((norm_quant_kernel<DT, GDT, KIND, 0>), grid, threads, 0, st, a);
 }
 
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -282,7 +297,7 @@ extern "C" int moe355_dynamic_mx_quant(const void* x, int x_dtype, int64_t rows,
     if (!x || !codes || !scale) return MOE355_E_ARG;
     if (!aligned(x, 16) || !aligned(codes, 4)) return MOE355_E_SHAPE;
     const int64_t pieces = rows * (cols / 8), groups = (pieces + kThreads - 1) / kThreads;
-    if (groups > 0x7fffffff) return MOE355_E_SHAPE;
+    if (groups > kMostThreads / kThreads) return MOE355_E_SHAPE;
 #define MOE355_MXQ(D_)                                                                                                   \
     hipLaunchKernelGGL(mx_quant_kernel<D_>, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, (const char*)x, \
                        pieces, (uint32_t*)codes, scale)
@@ -302,7 +317,7 @@ extern "C" int moe355_mx_dequant(const uint8_t* codes, const uint8_t* scale, int
     if (!codes || !scale || !out) return MOE355_E_ARG;
     if (!aligned(out, 16) || !aligned(codes, 4)) return MOE355_E_SHAPE;
     const int64_t pieces = rows * (cols / 8), groups = (pieces + kThreads - 1) / kThreads;
-    if (groups > 0x7fffffff) return MOE355_E_SHAPE;
+    if (groups > kMostThreads / kThreads) return MOE355_E_SHAPE;
 #define MOE355_MXD(D_)                                                                                            \
     hipLaunchKernelGGL(mx_dequant_kernel<D_>, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream,        \
                        (const uint32_t*)codes, scale, pieces, (char*)out)
@@ -320,7 +335,7 @@ extern "C" int moe355_add_rms_norm_quant(const void* x1, const void* x2, const v
     if (rows < 0 || cols <= 0 || (x_dtype != MOE355_DT_BF16 && x_dtype != MOE355_DT_F16)) return MOE355_E_ARG;
     if (weight_dtype != x_dtype && weight_dtype != MOE355_DT_F32) return MOE355_E_ARG;
     if (kind < MOE355_NORM_PLAIN || kind > MOE355_NORM_MXFP4 || !(epsilon >= 0.0)) return MOE355_E_ARG;
-    if (rows > 0x7fffffff || cols > (int64_t)1 << 20 || cols % (kind == MOE355_NORM_MXFP4 ? 32 : 8)) return MOE355_E_SHAPE;
+    if (cols > (int64_t)1 << 20 || rows > kMostThreads / norm_shape(cols).threads || cols % (kind == MOE355_NORM_MXFP4 ? 32 : 8)) return MOE355_E_SHAPE;
     if (rows == 0) return MOE355_OK;
     if (!x1 || !gamma || (kind != MOE355_NORM_PLAIN ? !q || !scale : !y)) return MOE355_E_ARG;
     if (!aligned(x1, 16) || !aligned(x2, 16) || !aligned(x, 16) || !aligned(y, 16) || !aligned(q, 8) || !aligned(gamma, 16) ||
