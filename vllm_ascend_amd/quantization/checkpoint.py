@@ -44,6 +44,8 @@ def moe_weight_loader(param: torch.nn.Parameter, loaded_weight: torch.Tensor, we
     if tuple(src.shape) != tuple(dst.shape):
         raise ValueError(f"{weight_name} (expert {expert_id}, {shard_id}): checkpoint shape {tuple(src.shape)} "
                          f"does not fit the parameter slice {tuple(dst.shape)}")
+    if dst.dtype == torch.uint8 and src.dtype.is_floating_point and src.element_size() == 1:
+        src = src.view(torch.uint8)  # MXFP4 codes or E8M0 scales under the name of their type: the bytes, not the numbers
     dst.copy_(src.to(dst.dtype))
     return True if return_success else None
 
