@@ -867,6 +867,8 @@ def _scale_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
 
 def _flat(t: torch.Tensor, name: str, alignment: int = 16) -> torch.Tensor:
     """Contiguous, on the GPU, and starting where the kernels' wide loads may start (a view into another tensor need not)."""
+    if t.is_cuda and t.is_contiguous() and t.data_ptr() % alignment == 0:
+        return t
     t = _dev(t, name)
     return t if t.data_ptr() % alignment == 0 else t.clone()
 
@@ -883,10 +885,11 @@ def _call(index: int, name: str, *args) -> None:
         check(rc, name)
 
 
-def _on(index: int, **others) -> None:
-    for name, t in others.items():
+def _on(index: int, *others) -> None:
+    for t in others:
         if t is not None and t.get_device() != index:
-            raise RuntimeError(f"{name} is on {t.device}, the rows on device {index}")
+            raise RuntimeError(f"operands on different devices: the rows on device {index}, a {tuple(t.shape)} {t.dtype} tensor on "
+                               f"{t.device}")
 
 
 def _rows_of(x: torch.Tensor, op: str, multiple: int) -> tuple[int, int]:
@@ -919,7 +922,7 @@ def mx_dequant(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = to
         raise ValueError(f"mx_dequant: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
     codes, scale = _flat(codes, "codes", 4), _dev(scale, "scale")
     index = codes.get_device()
-    _on(index, scale=scale)
+    _on(index, scale)
     out = torch.empty((*lead, half * 2), dtype=dtype, device=codes.device)
     _call(index, "moe355_mx_dequant", codes.data_ptr(), scale.data_ptr(), rows, half * 2, out.data_ptr(), _DT[dtype])
     return out
@@ -931,8 +934,9 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
     op = "add_rms_norm_quant"
     dtype = _half_dtype(x1.dtype)
     rows, cols = _rows_of(x1, op, MX_BLOCK if kind == NORM_MXFP4 else 8)
-    lead = x1.shape[:-1]
-    if x2 is not None and (x2.shape != x1.shape or x2.dtype != dtype):
+    shape = x1.shape
+    lead = shape[:-1]
+    if x2 is not None and (x2.dtype is not dtype or x2.shape != shape):
         raise ValueError(f"{op}: x2 {tuple(x2.shape)} {x2.dtype} does not match x1 {tuple(x1.shape)} {dtype}")
     wide = gamma.dtype is torch.float32
     if not (wide or gamma.dtype is dtype) or gamma.shape != (cols,):
@@ -945,12 +949,12 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
     x2 = None if x2 is None else _flat(x2, "x2")
     gamma, beta = _flat(gamma, "gamma"), None if beta is None else _flat(beta, "beta")
     index, dev = x1.get_device(), x1.device
-    _on(index, x2=x2, gamma=gamma, beta=beta)
+    _on(index, x2, gamma, beta)
     y = torch.empty_like(x1)
     x = torch.empty_like(x1) if x2 is not None else None
     q = scale = None
     if kind == NORM_INT8:
-        q = torch.empty(x1.shape, dtype=torch.int8, device=dev)
+        q = torch.empty_like(x1, dtype=torch.int8)
         scale = torch.empty(lead, dtype=torch.float32, device=dev)
     elif kind == NORM_MXFP4:
         q = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
@@ -978,7 +982,7 @@ def format_cast_mx(codes: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tens
     if scale.shape != (E, n, k // MX_BLOCK):
         raise ValueError(f"format_cast_mx: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
     codes, scale = _flat(codes, "weight"), _dev(scale, "scale")
-    _on(codes.get_device(), scale=scale)
+    _on(codes.get_device(), scale)
     out = torch.empty_like(codes)
     out_scale = torch.empty((E, n, mx_scale_columns(k)), dtype=torch.uint8, device=codes.device)
     _call(codes.get_device(), "moe355_format_cast_mx", codes.data_ptr(), scale.data_ptr(), E, n, k, out.data_ptr(),
@@ -1036,7 +1040,7 @@ def _mx_product(op, entry, x, x_scale, weight, weight_scale, group_list, group_l
     if group_list is not None:
         group_list = _gl(group_list)
     index = x.get_device()
-    _on(index, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, row_map=row_map)
+    _on(index, x_scale, weight, weight_scale, group_list, row_map)
     list_type = _gl_type(group_list_type)
 
     def call(*outputs):
@@ -1096,8 +1100,7 @@ def mx_experts(x, x_scale, topk_ids, topk_weights, w13, w13_scale, w2, w2_scale,
     w13, w13_scale = _flat(w13, "w13"), _flat(w13_scale, "w13_scale")
     w2, w2_scale, index = _flat(w2, "w2"), _flat(w2_scale, "w2_scale"), x.get_device()
     topk_ids, topk_weights = _dev(topk_ids, "topk_ids"), _dev(topk_weights, "topk_weights")
-    _on(index, x_scale=x_scale, topk_ids=topk_ids, topk_weights=topk_weights, w13=w13, w13_scale=w13_scale, w2=w2,
-        w2_scale=w2_scale, residual=residual)
+    _on(index, x_scale, topk_ids, topk_weights, w13, w13_scale, w2, w2_scale, residual)
     k, dev = topk_ids.shape[1], x.device
     out = torch.empty((T, H), dtype=dtype, device=dev)
     tokens = (torch.empty if T else torch.zeros)((E,), dtype=torch.int64, device=dev)
