@@ -8,7 +8,7 @@ HELD = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 def quantise(v):
     """[..., K] numbers -> (code of every value 0..15, scale bytes [..., K / 32])."""
     v = np.asarray(v, dtype=np.float64)
-    b = v.reshape(*v.shape[:-1], -1, 32)
+    b = v.reshape(*v.shape[:-1], v.shape[-1] // 32, 32)
     largest = np.abs(b).max(-1)
     finite = np.isfinite(largest)
     safe = np.where(finite & (largest > 0), largest, 1.0)

@@ -736,3 +736,42 @@ def test_products_captured_and_replayed_on_two_streams(K):
         torch.cuda.synchronize()
         for _, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("E,rows,kind", [(300, 40, "zipf"), (300, 299, "even"), (1100, 9, "even"), (700, 650, "one"), (2, 1, "even"),
+                                         (256, 255, "zipf"), (257, 200, "zipf"), (65, 64, "even")])
+@pytest.mark.parametrize("list_type", [0, 1])
+def test_fewer_rows_than_experts(K, E, rows, kind, list_type):
+    say("few rows", E, rows, kind, list_type)
+    N, Kd = 64, 576
+    rng, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, kind)
+    counts = rng.permutation(counts)
+    counts[counts.argmax()] -= 1  # a row behind the last group
+    used = int(counts.sum())
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    gl = dev(np.asarray(counts if list_type else counts.cumsum()).astype(np.int64))
+    check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, gl, list_type),
+               ref.products(ref.values(xc, xs), ref.values(wc, ws), counts), used)
+
+
+@pytest.mark.parametrize("list_type,gl,counts", [
+    (1, {3: -9, 4: 7, 90: 1 << 50, 200: 4, 299: -1}, {4: 7, 90: 33}),
+    (1, {0: 40, 7: 40, 299: 40}, {0: 40}),
+    (0, [(0, -5), (10, 3), (100, 1 << 50)], {10: 3, 100: 37}),
+    (0, [(0, 40), (299, 41)], {0: 40}),
+    (1, {}, {}), (0, [], {})])
+def test_fewer_rows_than_experts_and_lists_out_of_range(K, list_type, gl, counts):
+    say("few rows, lists out of range", list_type, gl)
+    E, N, Kd, rows = 300, 64, 64, 40
+    _, _, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    given, want = np.zeros(E, dtype=np.int64), np.zeros(E, dtype=np.int64)
+    for e, n in gl.items() if list_type else gl:
+        if list_type:
+            given[e] = n
+        else:
+            given[e:] = n
+    for e, n in counts.items():
+        want[e] = n
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, dev(given), list_type),
+               ref.products(ref.values(xc, xs), ref.values(wc, ws), want), int(want.sum()))

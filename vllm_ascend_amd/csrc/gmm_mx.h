@@ -115,6 +115,46 @@ __device__ __forceinline__ void mx_expert_rows(const MxArgs& a, int e, int lane,
     row1 = row1 < row0 ? row0 : row1 > a.rows ? a.rows : row1;
 }
 
+// With fewer rows than experts: the expert that has rows and `index` others that have some in front of it, and its rows.  No such
+// expert: false.  Every lane of a wavefront calls it.
+__device__ __forceinline__ bool mx_find_expert(const MxArgs& a, int index, int lane, int& e, int64_t& row0, int64_t& row1)
+{
+    const int32_t rows = (int32_t)a.rows;  // below 2^15, so that 32 bits hold the sum of the list
+    auto cut = [&](int64_t n) { return (int32_t)(n < 0 ? 0 : n < rows ? n : rows); };
+    int seen = 0;
+    int32_t before = 0;
+    for (int base = 0; base < a.E; base += 256) {
+        int32_t n[4], from[4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + 64 * j + lane;
+            n[j] = i < a.E ? cut(a.group_list[i]) : 0;
+            if (a.gl_type == MOE355_GL_CUMSUM) from[j] = i > 0 && i < a.E ? cut(a.group_list[i - 1]) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (a.gl_type == MOE355_GL_CUMSUM) n[j] = n[j] > from[j] ? n[j] - from[j] : 0;
+            const uint64_t has = __ballot(n[j] > 0);
+            const int here = __builtin_popcountll(has);
+            const int32_t inc = wave_scan_inclusive_i32(n[j]);
+            if (index < seen + here) {
+                const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+                const int who = __builtin_ctzll(__ballot(n[j] > 0 && rank == index - seen));
+                const int32_t size = __builtin_amdgcn_readlane(n[j], who);
+                const int32_t at = a.gl_type == MOE355_GL_CUMSUM ? __builtin_amdgcn_readlane(from[j], who)
+                                                                : before + __builtin_amdgcn_readlane(inc, who) - size;
+                e = base + 64 * j + who;
+                row0 = at < rows ? at : rows;
+                row1 = at + size < rows ? at + size : rows;
+                return row0 < row1;
+            }
+            seen += here;
+            before += __builtin_amdgcn_readlane(inc, 63);
+        }
+    }
+    return false;
+}
+
 // silu(g) u from its definition in 64 bits, rounded once
 __device__ __forceinline__ float swiglu_f64(float g, float u)
 {

@@ -21,21 +21,28 @@ __global__ __launch_bounds__(256) void mx_format_kernel(const uint8_t* __restric
         for (int64_t j = nb; j < 4; ++j) to_scale[(tile * windows + window) * 256 + lane * 4 + j] = 0;
 }
 
-// Few rows an expert: a workgroup has 64 channels of an expert and its rows, 32 at a time (every gridDim.z-th 32); its wavefronts
+// Few rows an expert: a workgroup has 64 channels of an expert and its rows, 32 at a time (every gridDim.z-th 32).  With fewer rows
+// than experts it looks for its expert among those that have some, so that nothing is launched for the others (one token, 8 of 128
+// experts of 2048 -> 2 x 768: 10.3 -> 5.6 us, of 256 of 7168 -> 2 x 2048: 34.8 -> 21.7).  Its wavefronts
 // have a part of K each and add their sums through LDS.  Three wavefronts a SIMD (168 registers), which is why the form of 64 rows
 // is not here.
 template <int EPI, int DT>
-__global__ __launch_bounds__(512, 3) void gmm_mx_stream_kernel(MxArgs a)
+__global__ __launch_bounds__(256, 3) void gmm_mx_stream_kernel(MxArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) float mx_parts[];
-    const int e = blockIdx.y, lane = threadIdx.x & 63;
-    // an expert without rows: seen before anything else is read
-    if (a.group_list) {
-        const int64_t n = a.group_list[e];
-        if (n <= (a.gl_type == MOE355_GL_CUMSUM && e > 0 ? a.group_list[e - 1] : 0)) return;
-    }
+    const int lane = threadIdx.x & 63;
+    int e = blockIdx.y;
     int64_t row0, row1;
-    mx_expert_rows(a, e, lane, row0, row1);
+    if (a.group_list && a.rows < a.E) {
+        if (!mx_find_expert(a, blockIdx.y, lane, e, row0, row1)) return;
+    } else {
+        // an expert without rows: seen before anything else is read
+        if (a.group_list) {
+            const int64_t n = a.group_list[e];
+            if (n <= (a.gl_type == MOE355_GL_CUMSUM && e > 0 ? a.group_list[e - 1] : 0)) return;
+        }
+        mx_expert_rows(a, e, lane, row0, row1);
+    }
     if (row0 + 32 * (int64_t)blockIdx.z >= row1) return;
     const int tiles = (int)(a.N / 32), windows = (int)((a.K + 255) / 256);
     MxStream<EPI, DT> s = {a, mx_parts, lane, lane >> 5};
@@ -59,13 +66,14 @@ void launch_stream(const MxArgs& a, hipStream_t st)
     const int64_t pairs = (a.N / 32 + 1) / 2, windows = (a.K + 255) / 256, experts = a.rows < a.E ? a.rows : a.E;
     // chunks of 32 rows side by side, twice as many as an expert has on average
     const int64_t chunks = (2 * a.rows + 32 * a.E - 1) / (32 * a.E), most = (a.rows + 31) / 32, z = chunks < most ? chunks : most;
-    // Wavefronts that share a K: as many as it takes to give every compute unit 12 of them, up to 8 of a window each at least; with
-    // 14 windows and more two or four anyway, since then a workgroup's start is less of it.  us with 1 / 2 / 4: 64 tokens, 256
-    // experts of 7168 -> 2 x 2048 (28 windows) 497 / 493 / 487, of 2048 -> 7168 (8 windows) 258 / 255 / 276; 128 experts of 2048
-    // -> 2 x 768 33.5 / 34.7 / 38.2, one token of it 7.7 / 7.1 / 7.5; a row of 7168 -> 4096 10.9 / 8.1 / 7.4.
+    // Wavefronts that share a K: two or four from 14 and 28 windows on, where a workgroup's start is less of it, and as long as there
+    // are no more wavefronts than compute units; more than four are slower (fewer workgroups fit a compute unit).  us with
+    // 1 / 2 / 4 / 8: 64 tokens, 256 experts of 7168 -> 2 x 2048 (28 windows) 497 / 493 / 487 / -, of 2048 -> 7168 (8 windows)
+    // 258 / 255 / 276 / -; 4 tokens, 128 experts of 2048 -> 2 x 768 10.3 / 10.9 / 11.9 / 17.8, one token (192 workgroups) 5.7 / 5.6 /
+    // 5.9 / 7.2; a row of 7168 -> 4096 (64 workgroups) 7.9 / 6.6 / 6.2 / 6.9, 32 rows 12.5 / 10.3 / 9.4 / 11.9.
     int waves = windows >= 28 ? 4 : windows >= 14 ? 2 : 1;
-    while (waves < 8 && pairs * experts * z * waves < 256 * 12 && 2 * waves <= windows) waves *= 2;
-    hipLaunchKernelGGL((gmm_mx_stream_kernel<EPI, DT>), dim3((unsigned)pairs, (unsigned)a.E, (unsigned)z), dim3(64 * waves),
+    while (waves < 4 && pairs * experts * z * waves <= 256 && 2 * waves <= windows) waves *= 2;
+    hipLaunchKernelGGL((gmm_mx_stream_kernel<EPI, DT>), dim3((unsigned)pairs, (unsigned)experts, (unsigned)z), dim3(64 * waves),
                        (waves - 1) * 32 * 64 * 4, st, a);
 }
 
@@ -94,7 +102,7 @@ MxForm mx_form(int64_t rows, int64_t n, int num_experts, bool swiglu, bool group
     // of 32 rows x 64 channels, and for fewer than 4 rows an expert.  us streamed / tiles: 8 experts of 1024 -> 2 x 1408, 64 / 128 /
     // 256 tokens of 2 slots 7.6 / 10.9 / 18.3 against 7.8 / 10.5 / 13.1 (352, 352, 704 workgroups), of 1408 -> 1024 5.1 / - / 6.1
     // against 6.3 / - / 9.9; one expert of 7168 -> 4096, 128 / 256 / 512 / 1024 rows 10.7 / 19.2 / 30.0 / 57.2 against 26.6 /
-    // 32.3 / 33.7 / 36.5.  128 experts of 2048 -> 2 x 768, 4 / 16 / 64 / 256 tokens of 8 slots 11.8 / 26.5 / 34.6 / 39.5 against
+    // 32.3 / 33.7 / 36.5.  128 experts of 2048 -> 2 x 768, 4 / 16 / 64 / 256 tokens of 8 slots 10.5 / 26.1 / 34.6 / 39.5 against
     // 14.8 / 27.7 / 34.7 / 39.0; skewed (Zipf(1.1)) 64 / 256 tokens 25.0 / 64.4 against 27.2 / 41.3, 256 experts of 7168 -> 2 x
     // 2048 128 / 512 tokens 249 / 690 against 189 / 317: a hot expert's many rows go through its few workgroups.
     const int64_t pairs = swiglu ? n / 64 : (n / 32 + 1) / 2, chunks = (rows + 32 * (int64_t)num_experts - 1) / (32 * (int64_t)num_experts);
