@@ -139,12 +139,19 @@ int gmm2_w4_pairs(const int8_t* x, const float* x_scale, const int32_t* topk_ids
                   int out_dtype, hipStream_t st);
 
 // moe355_route_map with the tile maps of the two products (nspecs of them, at most 2) built by the same launch where it
-// is one launch (one_launch_map; returns 1 in *built then), which also clears zeros_per_pair words for every pair
+// is one launch (one_launch_map; returns 1 in *built then), which also clears zeros_per_pair words for every pair.  quant: rows to
+// quantise on the way, bf16 or fp16 (16-byte aligned, cols a multiple of 32)
+struct MxQuantJob {
+    const void* x;
+    int dtype;
+    int64_t rows, cols;
+    uint8_t *codes, *scale;
+};
 bool one_launch_map(int64_t pairs, int num_experts);
 int route_map_impl(const int32_t* expert_idx, int64_t num_tokens, int top_k, int num_experts, int tokens_num_type,
                    int32_t* expanded_row_idx, int32_t* row_token, int64_t* expert_tokens, void* workspace,
                    size_t workspace_bytes, const TileSpec* specs, int nspecs, bool* built, void* stream, uint32_t* zeros = nullptr,
-                   int zeros_per_pair = 0);
+                   int zeros_per_pair = 0, const MxQuantJob* quant = nullptr);
 
 // ------------------------------------------------------------------ a few tokens (few.hip)
 // n / d for n and d below 2^16 in one multiplication (an integer division is about 25 instructions, one after the other)

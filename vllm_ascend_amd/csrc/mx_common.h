@@ -80,4 +80,16 @@ __device__ __forceinline__ void load8(const void* p, float (&v)[8])
     }
 }
 
+// Eight values a thread, piece i of `pieces`, a block of 32 by four neighbouring lanes.  (Whole blocks: a multiple of four pieces.)
+template <int DT>
+__device__ __forceinline__ void mx_quant_piece(const char* x, int64_t i, int64_t pieces, uint32_t* codes, uint8_t* scale)
+{
+    if (i >= pieces) return;
+    float v[8];
+    load8<DT>(x + i * 8 * (DT == MOE355_DT_F32 ? 4 : 2), v);
+    const MxScale s = mx_scale(mx_largest_of_quad(v));
+    codes[i] = mx_quantise8(v, s);
+    if ((threadIdx.x & 3) == 0) scale[i >> 2] = (uint8_t)s.byte;
+}
+
 }  // namespace moe355

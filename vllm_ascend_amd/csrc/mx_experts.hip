@@ -1,4 +1,4 @@
-// All MXFP4 experts of a layer on a batch whose routing is known, as one call: quantisation of the tokens, index maps (and the list
+// All MXFP4 experts of a layer on a batch whose routing is known, as one call: index maps (with the tokens' quantisation and the list
 // of tiles where a product wants one, by the same launch), both products, combine.
 #include "gmm_mx.h"
 #include "layer_parts.h"
@@ -84,8 +84,8 @@ extern "C" int moe355_mx_experts(const void* x, const uint8_t* x_scale, int dtyp
     hipStream_t st = (hipStream_t)stream;
     int rc;
     const uint8_t *codes = (const uint8_t*)x, *scale = x_scale;
+    const MxQuantJob job = {x, dtype, T, H, b.codes, b.scale};
     if (!x_scale) {
-        if ((rc = moe355_dynamic_mx_quant(x, dtype, T, H, b.codes, b.scale, stream))) return rc;
         codes = b.codes;
         scale = b.scale;
     }
@@ -99,7 +99,7 @@ extern "C" int moe355_mx_experts(const void* x, const uint8_t* x_scale, int dtyp
         spec.max_tiles = (int)mx_most_tiles(R, E);
     }
     if ((rc = route_map_impl(topk_ids, T, top_k, E, 1, b.dst, b.row_token, expert_tokens, b.map_ws, b.map_bytes, &spec,
-                             b.tiles ? 1 : 0, &built, stream)))
+                             b.tiles ? 1 : 0, &built, stream, nullptr, 0, x_scale ? nullptr : &job)))
         return rc;
     const MxArgs up = {codes, scale, b.row_token, w13, w13_scale, expert_tokens, MOE355_GL_COUNT, R, T, H, 2 * I, E, swiglu_limit,
                        b.hidden, b.hidden_scale, false};

