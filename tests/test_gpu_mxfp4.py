@@ -775,3 +775,36 @@ def test_fewer_rows_than_experts_and_lists_out_of_range(K, list_type, gl, counts
     w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
     check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, dev(given), list_type),
                ref.products(ref.values(xc, xs), ref.values(wc, ws), want), int(want.sum()))
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [
+    (1, 8, 1, 64, 64), (3, 5, 3, 192, 320), (16, 4, 4, 1024, 704), (8, 300, 8, 448, 64), (1, 128, 8, 2048, 768), (2, 8, 2, 7168, 192),
+    (1, 2, 2, 64, 2048), (5, 16, 7, 576, 128), (1, 1, 1, 16384, 64), (4, 2048, 6, 320, 256), (7, 6, 5, 8192, 64),
+    # just past what the form takes: 17 tokens, 9 slots, 65 pairs
+    (17, 8, 2, 64, 64), (2, 16, 9, 64, 64), (13, 8, 5, 64, 64)])
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+def test_experts_of_a_few_tokens(K, T, E, k, H, I, dtype):
+    """The bits of the operators one after the other: ids that repeat, within a token too, ids outside, infinities and NaN in a row."""
+    say("few tokens", T, E, k, H, I, dtype)
+    rng = np.random.default_rng(T * 100 + E)
+    w13, s13 = ref.random_mx(rng, (E, 2 * I, H), 1)
+    w2, s2 = ref.random_mx(rng, (E, H, I), 1)
+    held = (*K.format_cast_mx(dev(ref.pack(w13)), dev(s13 - 5)), *K.format_cast_mx(dev(ref.pack(w2)), dev(s2 - 5)))
+    g = torch.Generator().manual_seed(T)
+    x, residual = (torch.randn(T, H, generator=g).to(dtype).to(DEV) for _ in range(2))
+    weights = torch.rand(T, k, generator=g).to(dtype).to(DEV)
+    ids = torch.from_numpy(rng.integers(0, E, (T, k)).astype(np.int32)).to(DEV)
+    outside, same = ids.clone(), torch.full_like(ids, E - 1)
+    outside.view(-1)[::3], outside.view(-1)[1::4] = -1, E
+    odd = x.clone()
+    odd[0, 0], odd[-1, 33] = float("inf"), float("nan")
+    for rows, chosen in ((x, ids), (x, outside), (x, same), (odd, ids)):
+        for limit, res in ((0.0, None), (0.5, residual)):
+            want, want_tokens = op_by_op(K, rows, None, chosen, weights, *held, limit, res)
+            for given in ((rows, None), K.dynamic_mx_quant(rows)):
+                out, tokens = K.mx_experts(*given, chosen, weights, *held, limit, res)
+                assert torch.equal(tokens, want_tokens)
+                assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=9.0), want.nan_to_num(nan=9.0))
+    if H * I * T * k < 1 << 24:  # against the formula
+        y = experts_ref(x, ids.cpu().numpy(), weights, ref.values(w13, s13 - 5), ref.values(w2, s2 - 5), dtype)
+        assert close(K.mx_experts(x, None, ids, weights, *held)[0], y, dtype, k)

@@ -1,7 +1,8 @@
-// All MXFP4 experts of a layer on a batch whose routing is known, as one call: index maps (with the tokens' quantisation and the list
-// of tiles where a product wants one, by the same launch), both products, combine.
+// All MXFP4 experts of a layer on a batch whose routing is known, as one call: a few tokens in two launches (mx_few.hip); otherwise index
+// maps (with the tokens' quantisation and the list of tiles where a product wants one, by the same launch), both products, combine.
 #include "gmm_mx.h"
 #include "layer_parts.h"
+#include "mx_few.h"
 
 namespace moe355 {
 namespace {
@@ -88,6 +89,15 @@ extern "C" int moe355_mx_experts(const void* x, const uint8_t* x_scale, int dtyp
     if (!x_scale) {
         codes = b.codes;
         scale = b.scale;
+    }
+    if (mx_few_takes(T, top_k, H, I)) {
+        const MxArgs up = {nullptr, nullptr, nullptr, w13, w13_scale, nullptr, MOE355_GL_COUNT, R, T, H, 2 * I, E, swiglu_limit,
+                           b.hidden, b.hidden_scale, false};
+        const MxArgs down = {b.hidden, b.hidden_scale, nullptr, w2, w2_scale, nullptr, MOE355_GL_COUNT, R, R, I, H, E, 0.0f, out,
+                             nullptr, false};
+        const MxFew few = {x, x_scale, x_scale != nullptr, topk_ids, (const uint16_t*)topk_weights, (const uint16_t*)residual, top_k,
+                           expert_tokens};
+        return mx_few(up, down, few, dtype, T, st);
     }
     TileSpec spec = {};
     bool built = false;
