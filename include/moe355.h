@@ -614,7 +614,7 @@ int moe355_format_cast_mx(const uint8_t *codes, const uint8_t *scale, int64_t nu
  * vllm_ascend/device/device_op.py:208-291).
  * Row r of the sorted rows is row row_token[r] of x (NULL: row r, x_rows = rows); one outside [0, x_rows) counts as zeros (x_rows > 0).
  * The group list (int64, meaning as above; NULL: one expert, all rows) is cut to [0, rows); rows behind the last group are left as they were.
- * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; x, w, out 16-byte aligned; x_rows * k / 2 below 4 GiB less
+ * k % 64 == 0, n % 32 == 0 (with SwiGLU 64), both at most 2^20; (rows / 128 + num_experts) * n / 256 below 2^24; x, w, out 16-byte aligned; x_rows * k / 2 below 4 GiB less
  * 1 MiB; the memory at x_scale has four bytes even where one row of k = 64 has two. */
 /* may be 0: no workspace is read then */
 size_t moe355_gmm_mx_workspace(int64_t rows, int64_t n, int num_experts, int swiglu);
@@ -628,7 +628,8 @@ int moe355_gmm_mx_swiglu_quant(const uint8_t *x, const uint8_t *x_scale, const i
 
 /* All MXFP4 experts of a layer on a batch whose routing is known: moe355_dynamic_mx_quant (x_scale NULL: x [T, hidden] of dtype;
  * otherwise x [T, hidden / 2] and x_scale [T, hidden / 32] are the quantised rows), moe355_route_map, moe355_gmm_mx_swiglu_quant,
- * moe355_gmm_mx and moe355_token_unpermute in one call, the same bits.  topk_ids [T, k], topk_weights [T, k] of dtype; residual
+ * moe355_gmm_mx and moe355_token_unpermute in one call, the same bits where fp32 holds the products' sums exactly (blocks of a row
+ * some powers of two apart; otherwise the order of a sum depends on the form that the sizes choose).  topk_ids [T, k], topk_weights [T, k] of dtype; residual
  * [T, hidden] of dtype or NULL; expert_tokens [E] receives the counts; out [T, hidden] of dtype (bf16 / fp16).  hidden and
  * intermediate are multiples of 64, E at most 2048, k at most 64. */
 size_t moe355_mx_experts_workspace(int64_t num_tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts,

@@ -808,3 +808,20 @@ def test_experts_of_a_few_tokens(K, T, E, k, H, I, dtype):
     if H * I * T * k < 1 << 24:  # against the formula
         y = experts_ref(x, ids.cpu().numpy(), weights, ref.values(w13, s13 - 5), ref.values(w2, s2 - 5), dtype)
         assert close(K.mx_experts(x, None, ids, weights, *held)[0], y, dtype, k)
+
+
+@pytest.mark.parametrize("E,N,Kd,rows", [(1, 64, 7168, 1), (1, 4096, 4096, 20), (4, 128, 2048, 9), (2, 512, 4096, 700),
+                                        (1, 1024, 8192, 300), (600, 64, 1024, 4000)])
+def test_sums_that_32_bits_do_not_hold(K, E, N, Kd, rows):
+    """Blocks up to 2^40 apart.  Every addition of at most K, to a sum of 24 bits that may be cut off instead of rounded, is off by
+    at most 2^-23 of what the magnitudes add up to, and the result by half a step of bf16 on top: its steps are 2^-7 of the power of
+    two below a value, half of one is at most 2^-8 of the value."""
+    say("inexact sums", E, N, Kd, rows)
+    rng, counts, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    xs = rng.integers(107, 147, xs.shape).astype(np.uint8)
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    got = K.gmm_mx(dev(ref.pack(xc)), dev(xs), w, s, dev(counts.astype(np.int64)), 1).double().cpu().numpy()
+    x, wv = ref.values(xc, xs), ref.values(wc, ws)
+    want = ref.products(x, wv, counts)
+    bound = np.abs(want) * 2.0 ** -8 * 1.001 + Kd * 2.0 ** -23 * ref.products(np.abs(x), np.abs(wv), counts)
+    assert (np.abs(got - want) <= bound).all()

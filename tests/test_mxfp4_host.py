@@ -265,3 +265,5 @@ def test_launches_larger_than_there_are(lib):
     norm = lambda rows, cols: lib.moe355_add_rms_norm_quant(P, P, P, None, 1, 1, rows, cols, 1e-6, 1, P, P, P, P, None)
     assert norm(1 << 26, 512) == -2 and norm(1 << 22, 16384) == -2
     assert lib.moe355_format_cast_mx(P, P, 32768, 1 << 16, 64, P, P, None) == -2
+    gmm = lambda rows, n: lib.moe355_gmm_mx(P, P, P, 4, P, P, P, 1, rows, 64, n, 2, P, 1, None, 0, None)
+    assert gmm((1 << 31) - 1, 1 << 20) == -2

@@ -343,7 +343,6 @@ int launch_mx_tiled(const MxArgs& a, bool swiglu, int out_dtype, MxForm form, co
     const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8, tiles = (a.rows + kTileRows - 1) / kTileRows;
     const bool direct = form == MX_TILES && a.group_list;
     const int64_t most = (form == MX_LISTED ? mx_most_tiles(a.rows, a.E) : tiles) * columns, groups = (most + 7) / 8 * 8;
-    if (groups > 0xffffffff / kThreads) return MOE355_E_SHAPE;  // a launch has at most 2^32 - 1 threads
     const dim3 grid = direct ? dim3((unsigned)columns, (unsigned)a.E, (unsigned)tiles) : dim3((unsigned)groups);
 #define MOE355_MXT(E_, D_)                                                                                       \
     do {                                                                                                         \
