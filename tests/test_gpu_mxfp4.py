@@ -780,8 +780,9 @@ def test_fewer_rows_than_experts_and_lists_out_of_range(K, list_type, gl, counts
 @pytest.mark.parametrize("T,E,k,H,I", [
     (1, 8, 1, 64, 64), (3, 5, 3, 192, 320), (16, 4, 4, 1024, 704), (8, 300, 8, 448, 64), (1, 128, 8, 2048, 768), (2, 8, 2, 7168, 192),
     (1, 2, 2, 64, 2048), (5, 16, 7, 576, 128), (1, 1, 1, 16384, 64), (4, 2048, 6, 320, 256), (7, 6, 5, 8192, 64),
-    # just past what the form takes: 17 tokens, 9 slots, 65 pairs
-    (17, 8, 2, 64, 64), (2, 16, 9, 64, 64), (13, 8, 5, 64, 64)])
+    (17, 8, 2, 64, 64), (13, 8, 5, 64, 64), (32, 16, 4, 512, 256), (16, 128, 8, 192, 64),
+    # just past what the form takes: 33 tokens, 9 slots, 130 pairs, more weights or more read again than it is worth
+    (33, 8, 2, 64, 64), (2, 16, 9, 64, 64), (26, 8, 5, 64, 64), (8, 64, 6, 2048, 1408), (32, 8, 2, 1024, 1408)])
 @pytest.mark.parametrize("dtype", HALF, ids=str)
 def test_experts_of_a_few_tokens(K, T, E, k, H, I, dtype):
     """The bits of the operators one after the other: ids that repeat, within a token too, ids outside, infinities and NaN in a row."""

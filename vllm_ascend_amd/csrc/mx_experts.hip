@@ -90,7 +90,7 @@ extern "C" int moe355_mx_experts(const void* x, const uint8_t* x_scale, int dtyp
         codes = b.codes;
         scale = b.scale;
     }
-    if (mx_few_takes(T, top_k, H, I)) {
+    if (mx_few_takes(T, top_k, H, I, E)) {
         const MxArgs up = {nullptr, nullptr, nullptr, w13, w13_scale, nullptr, MOE355_GL_COUNT, R, T, H, 2 * I, E, swiglu_limit,
                            b.hidden, b.hidden_scale, false};
         const MxArgs down = {b.hidden, b.hidden_scale, nullptr, w2, w2_scale, nullptr, MOE355_GL_COUNT, R, R, I, H, E, 0.0f, out,

@@ -15,7 +15,7 @@ struct MxFew {
     int top_k;
     int64_t* expert_tokens;
 };
-bool mx_few_takes(int64_t tokens, int top_k, int64_t hidden, int64_t intermediate);
+bool mx_few_takes(int64_t tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts);
 // up: to hidden rows in the order of the pairs, which down reads; down.out: the result [tokens, N]
 int mx_few(const MxArgs& up, const MxArgs& down, const MxFew& f, int dtype, int64_t tokens, hipStream_t st);
 

@@ -3,12 +3,12 @@
 //
 //   few_up_kernel    a workgroup has a pair and 32 gate channels with their 32 up channels.  It quantises the pair's token itself,
 //                    into LDS, while its first weights are on their way, and its wavefronts share K.
-//   few_down_kernel  a workgroup has 64 channels of a token and all its slots, a wavefront or more each, so that the token's rows
+//   few_down_kernel  a workgroup has 32 channels of a token and all its slots, a wavefront or more each, so that the token's rows
 //                    meet in LDS and leave as one: the combine, and the counts of the experts by one more row of workgroups.
 //
 // The 32 columns of a product all have the pair's row; lanes 0 and 32 hold what is wanted.  An expert that several tokens chose is
-// read for each of them, which is what ends the use (mx_few_takes).
-#include "gmm_mx_stream.h"
+// read for each of them, which is what ends the use (mx_few_takes).  One token through 8 of 128 experts of 2048 x 768 takes 12 us on
+// the GPU (20 MB: 4 us; the two launches by themselves, behind an idle GPU, 6.8 and 5.8).
 #include "mx_few.h"
 
 namespace moe355 {
@@ -16,47 +16,124 @@ namespace {
 
 constexpr int kFewWaves = 8;
 
-// 64 channels (two blocks) of this wavefront's windows; fetch(w) asks for a window's row, b(w, j) and scale(w) hand it over
-template <class Stream, class Row>
-__device__ __forceinline__ void few_stream(const Stream& s, typename Stream::Weights (&held)[2], const Row& row, v16f (&acc)[2])
-{
-    auto multiply = [&](const typename Stream::Weights& w, int at, int nb) {
-        const int scale = row.scale(at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < nb) {
-                const v4i b = row.codes(at, nb, j);
-                acc[0] = mfma_mx(w.a[0][j], b, acc[0], w.s[0], scale, j);
-                acc[1] = mfma_mx(w.a[1][j], b, acc[1], w.s[1], scale, j);
-            }
+// NB blocks of 32 channels of an expert, the windows [begin, end) of their K
+template <int NB>
+struct FewBlocks {
+    __amdgpu_buffer_rsrc_t w[NB], ws[NB];
+    int lane, half, full, tail, begin, end;  // whole windows of the row, steps of a last, shorter one
+
+    struct Weights {
+        v4i a[NB][4];
+        int s[NB];
     };
-    int w = s.w_begin;
-    for (; w + 1 < s.w_end; w += 2) {
-        s.template fetch_weights<false>(w + 1, held[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(held[0], w, 4);  // (the last window, the only one that may be short, comes below or second)
-        __builtin_amdgcn_sched_barrier(0);
-        s.template fetch_weights<false>(w + 2, held[0]);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(held[1], w + 1, w + 1 < s.full ? 4 : s.tail);
-        __builtin_amdgcn_sched_barrier(0);
+    // the `part`-th of `parts` parts
+    __device__ __forceinline__ FewBlocks(const MxArgs& a, int e, const int (&block)[NB], int part, int parts)
+    {
+        const int64_t tiles = a.N / 32, steps = a.K / 64;
+        const int windows = (int)((steps + 3) / 4), share = (windows + parts - 1) / parts;
+        lane = threadIdx.x & 63;
+        half = lane >> 5;
+        full = (int)(steps >> 2);
+        tail = (int)(steps & 3);
+        begin = part * share < windows ? part * share : windows;
+        end = begin + share < windows ? begin + share : windows;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int64_t at = e * tiles + block[i];
+            w[i] = mx_buffer(a.w + at * steps * 1024, (uint32_t)steps * 1024);
+            ws[i] = mx_buffer(a.w_scale + at * windows * 256, (uint32_t)windows * 256);
+        }
     }
-    if (w < s.w_end) multiply(held[0], w, w < s.full ? 4 : s.tail);
-}
+    __device__ __forceinline__ int steps_of(int at) const { return at < full ? 4 : tail; }
+    __device__ __forceinline__ void fetch(int at, Weights& to) const
+    {
+        const int from = at < end ? at * 4096 + lane * 16 : 0x7ffff000;  // past the end: nothing is read
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to.a[i][j] = __builtin_amdgcn_raw_buffer_load_b128(w[i], from + j * 1024, 0, 0);
+            to.s[i] = __builtin_amdgcn_raw_buffer_load_b32(ws[i], at * 256 + lane * 4, 0, 0);
+        }
+    }
+    // `held`: the first window, asked for
+    template <class Row>
+    __device__ __forceinline__ void products(Weights (&held)[2], const Row& row, v16f (&acc)[NB]) const
+    {
+        typename Row::Held x[2];
+        row.fetch(begin, steps_of(begin), x[0]);
+        auto multiply = [&](const Weights& v, const typename Row::Held& r, int nb) {
+            const int scale = row.scale(r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < nb) {
+                    const v4i c = row.codes(r, nb, j);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) acc[i] = mfma_mx(v.a[i][j], c, acc[i], v.s[i], scale, j);
+                }
+        };
+        auto ask = [&](int at, int slot) {
+            fetch(at, held[slot]);
+            const int last = at < end ? at : end - 1;
+            row.fetch(last, steps_of(last), x[slot]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int at = begin;
+        for (; at + 1 < end; at += 2) {
+            ask(at + 1, 1);
+            multiply(held[0], x[0], 4);  // (the last window, the only one that may be short, is the second one or comes below)
+            __builtin_amdgcn_sched_barrier(0);
+            ask(at + 2, 0);
+            multiply(held[1], x[1], steps_of(at + 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (at < end) multiply(held[0], x[0], steps_of(at));
+    }
+};
 
 // A row in LDS: codes as they are, four scales a window and half of the lanes
 struct FewRow {
     const uint8_t* row;
     const int* scales;
     int half;
-    __device__ __forceinline__ v4i codes(int w, int nb, int j) const { return *(const v4i*)(row + (w * 8 + half * nb + j) * 16); }
-    __device__ __forceinline__ int scale(int w) const { return scales[w * 2 + half]; }
+    struct Held {
+        int at;
+    };
+    __device__ __forceinline__ void fetch(int at, int, Held& to) const { to.at = at; }
+    __device__ __forceinline__ v4i codes(const Held& h, int nb, int j) const { return *(const v4i*)(row + (h.at * 8 + half * nb + j) * 16); }
+    __device__ __forceinline__ int scale(const Held& h) const { return scales[h.at * 2 + half]; }
     // where block b of a row of `blocks` blocks has its scale, in bytes
     static __device__ __forceinline__ int place(int b, int blocks)
     {
         const int w = b >> 3, left = blocks - 8 * w, nb = left < 8 ? left / 2 : 4, in = b & 7, h = in >= nb;
         return (w * 2 + h) * 4 + in - h * nb;
     }
+};
+
+// A row in memory, asked for with the weights
+struct FewHidden {
+    __amdgpu_buffer_rsrc_t x, xs;
+    uint32_t from, scale_from, scale_end;
+    int half;
+    struct Held {
+        v4i b[4];
+        MxRowScales s;
+    };
+    __device__ __forceinline__ FewHidden(const MxArgs& a, int row, int half_) : half(half_)
+    {
+        scale_end = mx_scale_bytes(a) - 4;
+        x = mx_buffer(a.x, (uint32_t)(a.x_rows * (a.K / 2)));
+        xs = mx_buffer(a.x_scale, scale_end + 4);
+        from = (uint32_t)row * (uint32_t)(a.K / 2);
+        scale_from = (uint32_t)row * (uint32_t)(a.K / 32);
+    }
+    __device__ __forceinline__ void fetch(int at, int nb, Held& to) const
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to.b[j] = __builtin_amdgcn_raw_buffer_load_b128(x, from + (at * 8 + half * nb + j) * 16, 0, 0);
+        to.s.fetch(xs, scale_from + at * 8 + half * nb, scale_end);
+    }
+    __device__ __forceinline__ v4i codes(const Held& h, int, int j) const { return h.b[j]; }
+    __device__ __forceinline__ int scale(const Held& h) const { return h.s.get(); }
 };
 
 template <int DT>
@@ -69,18 +146,11 @@ __global__ __launch_bounds__(256) void few_up_kernel(MxArgs a, MxFew f)
     if (e < 0 || e >= a.E) return;
     int* const scales = (int*)few_lds;                         // [windows][2]
     float* const sums = (float*)few_lds + (2 * windows + 3) / 4 * 4;  // [waves - 1][2][32]
-    MxStream<MX_SWIGLU, DT> s = {a, nullptr, lane, half};
-    s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    s.waves = blockDim.x >> 6;
-    uint8_t* const row = (uint8_t*)(sums + (s.waves - 1) * 64);  // [K / 2], and a window's reach past it
-    const int part = (windows + s.waves - 1) / s.waves;
-    s.w_begin = s.wave * part < windows ? s.wave * part : windows;
-    s.w_end = s.w_begin + part < windows ? s.w_begin + part : windows;
-    s.t0 = blockIdx.x;
-    s.t1 = s.t0 + tiles / 2;
-    s.operands(e);
-    typename MxStream<MX_SWIGLU, DT>::Weights held[2];
-    s.template fetch_weights<false>(s.w_begin, held[0]);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    uint8_t* const row = (uint8_t*)(sums + (waves - 1) * 64);  // [windows][128]
+    const FewBlocks<2> s(a, e, {(int)blockIdx.x, (int)blockIdx.x + tiles / 2}, wave, waves);
+    FewBlocks<2>::Weights held[2];
+    s.fetch(s.begin, held[0]);
     __builtin_amdgcn_sched_barrier(0);
 
     const int64_t token = pair / f.top_k;
@@ -100,16 +170,16 @@ __global__ __launch_bounds__(256) void few_up_kernel(MxArgs a, MxFew f)
     }
     __syncthreads();
     v16f acc[2] = {};
-    few_stream(s, held, FewRow{row, scales, half}, acc);
-    if (s.waves > 1) {
-        if (s.wave > 0 && (lane & 31) == 0) {
-            float* p = sums + (s.wave - 1) * 64 + half * 32;
+    s.products(held, FewRow{row, scales, half}, acc);
+    if (waves > 1) {
+        if (wave > 0 && (lane & 31) == 0) {
+            float* p = sums + (wave - 1) * 64 + half * 32;
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] = acc[0][i], p[16 + i] = acc[1][i];
         }
         __syncthreads();
-        if (s.wave > 0) return;
-        for (int v = 0; v < s.waves - 1; ++v) {
+        if (wave > 0) return;
+        for (int v = 0; v < waves - 1; ++v) {
             const float* p = sums + v * 64 + half * 32;
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[0][i] += p[i], acc[1][i] += p[16 + i];
@@ -117,33 +187,16 @@ __global__ __launch_bounds__(256) void few_up_kernel(MxArgs a, MxFew f)
     }
     const MxBlock b = mx_swiglu(acc[0], acc[1], a.limit, true);
     if ((lane & 31) == 0) {
-        *(uint2*)((uint8_t*)a.out + pair * (a.N / 4) + s.t0 * 16 + 8 * half) = b.codes;
-        if (half == 0) a.out_scale[pair * (a.N / 64) + s.t0] = (uint8_t)b.scale;
+        *(uint2*)((uint8_t*)a.out + pair * (a.N / 4) + blockIdx.x * 16 + 8 * half) = b.codes;
+        if (half == 0) a.out_scale[pair * (a.N / 64) + blockIdx.x] = (uint8_t)b.scale;
     }
 }
-
-// A row in memory, read where it is used
-template <int EPI, int DT>
-struct FewHidden {
-    const MxStream<EPI, DT>& s;
-    uint32_t x, xs;
-    __device__ __forceinline__ v4i codes(int w, int nb, int j) const
-    {
-        return __builtin_amdgcn_raw_buffer_load_b128(s.xb, x + (w * 8 + s.half * nb + j) * 16, 0, 0);
-    }
-    __device__ __forceinline__ int scale(int w) const
-    {
-        MxRowScales r;
-        r.fetch(s.xsb, xs + w * 8 + s.half * (w < s.full ? 4 : s.tail), s.scale_end);
-        return r.get();
-    }
-};
 
 template <int DT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(MxArgs a, MxFew f, int parts)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
-    float* const sums = (float*)few_lds;  // [slots][parts][64]
+    float* const sums = (float*)few_lds;  // [slots][parts][32]
     const int tokens = gridDim.y - 1, k = f.top_k;
     if ((int)blockIdx.y == tokens) {
         if (blockIdx.x > 0) return;
@@ -154,40 +207,30 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(MxArgs a, MxFe
         }
         return;
     }
-    const int lane = threadIdx.x & 63, half = lane >> 5, tiles = (int)(a.N / 32), windows = (int)((a.K + 255) / 256);
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / parts;
     const int pair = blockIdx.y * k + slot, e = f.ids[pair];
     if (e >= 0 && e < a.E) {
-        MxStream<MX_HALF, DT> s = {a, nullptr, lane, half};
-        const int part = (windows + parts - 1) / parts, mine = wave - slot * parts;
-        s.w_begin = mine * part < windows ? mine * part : windows;
-        s.w_end = s.w_begin + part < windows ? s.w_begin + part : windows;
-        s.t0 = 2 * blockIdx.x;
-        s.t1 = s.t0 + 1 < tiles ? s.t0 + 1 : s.t0;
-        s.operands(e);
-        typename MxStream<MX_HALF, DT>::Weights held[2];
-        s.template fetch_weights<false>(s.w_begin, held[0]);
-        v16f acc[2] = {};
-        few_stream(s, held, FewHidden<MX_HALF, DT>{s, (uint32_t)pair * (uint32_t)(a.K / 2), (uint32_t)pair * (uint32_t)(a.K / 32)}, acc);
+        const FewBlocks<1> s(a, e, {(int)blockIdx.x}, wave - slot * parts, parts);
+        FewBlocks<1>::Weights held[2];
+        s.fetch(s.begin, held[0]);
+        v16f acc[1] = {};
+        if (s.begin < s.end) s.products(held, FewHidden(a, pair, half), acc);
         if ((lane & 31) == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float* p = sums + wave * 64 + 8 * (i / 4) + 4 * half + i % 4;
-                p[0] = acc[0][i];
-                p[32] = acc[1][i];
-            }
+            for (int i = 0; i < 16; ++i) sums[wave * 32 + 8 * (i / 4) + 4 * half + i % 4] = acc[0][i];
         }
     }
     __syncthreads();
     // the sequence of the combine: 16-bit rows times their weights, slot by slot in 32 bits, the residual last
-    const int64_t channel = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (threadIdx.x >= 64 || channel >= a.N) return;
+    const int64_t channel = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x >= 32) return;
     float out = 0.0f;
     for (int i = 0; i < k; ++i) {
         const int id = f.ids[blockIdx.y * k + i];
         if (id < 0 || id >= a.E) continue;
-        float v = sums[i * parts * 64 + threadIdx.x];
-        for (int p = 1; p < parts; ++p) v += sums[(i * parts + p) * 64 + threadIdx.x];
+        float v = sums[i * parts * 32 + threadIdx.x];
+        for (int p = 1; p < parts; ++p) v += sums[(i * parts + p) * 32 + threadIdx.x];
         const float product = half_to_f32<DT>(f.probs[blockIdx.y * k + i]) * half_to_f32<DT>(f32_to_half<DT>(v));
         out = out + product;
     }
@@ -198,17 +241,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(MxArgs a, MxFe
 
 }  // namespace
 
-bool mx_few_takes(int64_t tokens, int top_k, int64_t hidden, int64_t intermediate)
+bool mx_few_takes(int64_t tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts)
 {
-    // A wavefront for every slot of a token, a row of x in LDS; and no more than what an expert that is read for each of its pairs
-    // costs less than the launches do.  us on the GPU, here / sorted, and the pairs' products H I in millions: 128 experts of
-    // 2048 x 768, 1 / 4 / 8 / 16 tokens of 8 slots 13.5 / 22 / 31 / 53 against 17 / 25 / 35 / 46 (12 / 50 / 100 / 201); 8 of 1024 x
-    // 1408, 1 / 8 / 16 / 32 tokens of 2 slots 10.5 / 11.5 / 13.5 / 21.4 against 16 / 17.6 / 17.9 / 18.1 (3 / 23 / 46 / 92); 64 of
-    // 2048 x 1408, 4 / 8 tokens of 6 slots 29.5 / 42 against 29 / 40 (69 / 138); 256 of 7168 x 2048, 1 / 2 tokens of 8 slots 39.7 / 77
-    // against 41 / 71 (117 / 235); 8 of 4096 x 1024 that 4 tokens have all 24 against 21 (134); 16 tokens of 8 slots of 1024 x 512, 128
-    // pairs of 128 experts 25.4 against 24.5 (67).  The host gains 6 us of 23 in all of them.
-    return tokens <= 16 && top_k <= kFewWaves && tokens * top_k <= 64 && hidden <= 65536 &&
-           tokens * top_k * hidden * intermediate <= 125000000;
+    // A wavefront for every slot of a token, a row of x in LDS; and the launches that it saves are worth some 125 million weights of
+    // each projection in all, 50 million of them read again because several pairs have the same expert.  us on the GPU, here /
+    // sorted (the host gains 6 of 23 in all of them), and those two numbers: 128 experts of 2048 x 768, 1 / 4 / 8 / 16 tokens of 8
+    // slots 12 / 20.7 / 29.8 / 48.2 against 17 / 25 / 34.5 / 46.3 (13, 50, 100, 201; 0); 8 of 1024 x 1408, 1 / 8 / 16 / 32 tokens of 2
+    // slots 9.5 / 10.5 / 13.5 / 21.2 against 16 / 17.8 / 18 / 18.2 (3, 23, 46, 92; 0, 12, 35, 81); 64 of 2048 x 1408, 4 / 8 tokens of 6
+    // slots 26.4 / 40.5 against 28.3 / 38 (69, 138; 0); 256 of 7168 x 2048, 1 / 2 tokens of 8 slots 36.3 / 76 against 41 / 71.6 (117, 235;
+    // 0); 8 of 4096 x 1024 that 4 tokens have all 24.2 against 22.4 (134; 101); 128 of 1024 x 512, 16 tokens of 8 slots 22.7 against
+    // 25.2 (67; 0); 16 of 512 x 256, 32 tokens of 4 slots 11.8 against 15.6 (17; 15).
+    if (tokens > 32 || top_k > kFewWaves || tokens * top_k > 128 || hidden > 65536) return false;
+    const int64_t pairs = tokens * top_k, again = pairs > num_experts ? pairs - num_experts : 0;
+    return pairs * hidden * intermediate <= 125000000 && again * hidden * intermediate <= 50000000;
 }
 
 int mx_few(const MxArgs& up, const MxArgs& down, const MxFew& f, int dtype, int64_t tokens, hipStream_t st)
@@ -219,14 +264,15 @@ int mx_few(const MxArgs& up, const MxArgs& down, const MxFew& f, int dtype, int6
     int parts = 1;
     while (2 * parts * f.top_k <= kFewWaves && 2 * parts <= windows2) parts *= 2;
     const size_t lds = (size_t)((2 * windows + 3) / 4 * 4) * 4 + (waves - 1) * 64 * 4 + windows * 128;
-    const dim3 up_grid((unsigned)(up.N / 64), (unsigned)pairs), down_grid((unsigned)((down.N / 32 + 1) / 2), (unsigned)tokens + 1);
-    const size_t down_lds = (size_t)f.top_k * parts * 64 * 4;
+    const dim3 up_grid((unsigned)(up.N / 64), (unsigned)pairs), up_threads(64 * waves), down_threads(64 * f.top_k * parts);
+    const dim3 down_grid((unsigned)(down.N / 32), (unsigned)tokens + 1);
+    const size_t down_lds = (size_t)f.top_k * parts * 32 * 4;
     if (dtype == MOE355_DT_BF16) {
-        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_BF16>, up_grid, dim3(64 * waves), lds, st, up, f);
-        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_BF16>, down_grid, dim3(64 * f.top_k * parts), down_lds, st, down, f, parts);
+        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_BF16>, up_grid, up_threads, lds, st, up, f);
+        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_BF16>, down_grid, down_threads, down_lds, st, down, f, parts);
     } else {
-        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_F16>, up_grid, dim3(64 * waves), lds, st, up, f);
-        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_F16>, down_grid, dim3(64 * f.top_k * parts), down_lds, st, down, f, parts);
+        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_F16>, up_grid, up_threads, lds, st, up, f);
+        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_F16>, down_grid, down_threads, down_lds, st, down, f, parts);
     }
     return launch_status();
 }

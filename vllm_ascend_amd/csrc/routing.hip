@@ -483,8 +483,8 @@ __global__ __launch_bounds__(kMapThreads) void route_map_kernel(RouteMapArgs a)
 }
 
 // With the rows' MXFP4 form by the workgroups behind those of the maps: both only wait for what was there before, and a launch of
-// its own costs a small batch 3 us on the GPU and 3.6 on the host (one token through 8 of 128 experts 17.7 -> 16.1 us, 512 of 7168
-// through 256 470 -> 454).  Not beside MANY: its registers leave a compute unit one such workgroup, too few loads for the memory.
+// its own costs a small batch 2 to 3 us on the GPU and 3.6 on the host, a larger one what it takes (512 tokens of 7168 through 256
+// experts, Zipf(1.1), 470 -> 454 us).  Not beside MANY: its registers leave a compute unit one such workgroup, too few loads for the memory.
 template <int DT>
 __global__ __launch_bounds__(kMapThreads) void route_map_quant_kernel(RouteMapArgs a, MxQuantJob q)
 {
