@@ -826,3 +826,53 @@ def test_sums_that_32_bits_do_not_hold(K, E, N, Kd, rows):
     want = ref.products(x, wv, counts)
     bound = np.abs(want) * 2.0 ** -8 * 1.001 + Kd * 2.0 ** -23 * ref.products(np.abs(x), np.abs(wv), counts)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("E,rows", [(3, 2), (3, 9), (3, 900), (600, 4000)])
+def test_group_lists_at_the_ends_of_64_bits(K, E, rows):
+    say("group lists at the ends", E, rows)
+    N, Kd = 1600 if E == 3 else 64, 64
+    _, _, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    most, least = (1 << 63) - 1, -(1 << 63)
+    acc = ref.products(ref.values(xc, xs), ref.values(wc, ws), [0, rows] + [0] * (E - 2))
+    for list_type, gl in ((1, [least, most, most]), (0, [least, most, most]), (0, [0, most, least]), (1, [least, rows, least])):
+        gl = gl + [gl[-1]] * (E - 3)
+        check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, torch.tensor(gl, device=DEV), list_type), acc)
+
+
+@pytest.mark.parametrize("T", [3, 100])
+def test_experts_from_two_threads_and_streams(K, T):
+    """Calls at once on two streams, each thread with tensors of its own, against calls one after the other."""
+    import threading
+
+    say("two threads", T)
+    E, k, H, I = 8, 2, 512, 256
+    rng = np.random.default_rng(T)
+    w13, s13 = ref.random_mx(rng, (E, 2 * I, H), 1)
+    w2, s2 = ref.random_mx(rng, (E, H, I), 1)
+    held = (*K.format_cast_mx(dev(ref.pack(w13)), dev(s13 - 5)), *K.format_cast_mx(dev(ref.pack(w2)), dev(s2 - 5)))
+    inputs = []
+    for i in range(2):
+        g = torch.Generator().manual_seed(i)
+        inputs.append((torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV), None,
+                       torch.from_numpy(rng.integers(0, E, (T, k)).astype(np.int32)).to(DEV),
+                       torch.rand(T, k, generator=g).to(torch.bfloat16).to(DEV)))
+    want = [K.mx_experts(*a, *held) for a in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(K.mx_experts(*inputs[i], *held))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 20
+        assert all(torch.equal(o, want[i][0]) and torch.equal(n, want[i][1]) for o, n in got[i])

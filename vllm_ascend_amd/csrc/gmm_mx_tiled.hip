@@ -108,8 +108,9 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     if constexpr (GRID) {
         e = blockIdx.y;
         column = blockIdx.x;
-        const int64_t n = a.group_list[e], m = a.gl_type == MOE355_GL_CUMSUM ? n - (e > 0 ? a.group_list[e - 1] : 0) : n;
-        if (m <= (int64_t)blockIdx.z * kTileRows) return;
+        // an expert without rows for this workgroup: seen before anything else is read
+        const int64_t n = min(a.group_list[e], a.rows), last = a.gl_type == MOE355_GL_CUMSUM && e > 0 ? a.group_list[e - 1] : 0;
+        if (n - max(last, (int64_t)0) <= (int64_t)blockIdx.z * kTileRows) return;
         mx_expert_rows(a, e, lane, row0, row1);
         row0 += (int64_t)blockIdx.z * kTileRows;
         if (row0 >= row1) return;
