@@ -876,3 +876,24 @@ def test_experts_from_two_threads_and_streams(K, T):
     for i in range(2):
         assert len(got[i]) == 20
         assert all(torch.equal(o, want[i][0]) and torch.equal(n, want[i][1]) for o, n in got[i])
+
+
+@pytest.mark.parametrize("case", [(128, 1536, 2048, 512, "zipf"), (3, 1088, 576, 1900, "zipf"), (4, 704, 960, 2100, "zipf"),
+                                  (1, 512, 192, 1000, "even"), (600, 64, 320, 4000, "zipf"), (16, 128, 2048, 200, "zipf")], ids=str)
+def test_products_on_cold_caches(K, case):
+    """Rows and weights come late, out of the memory itself: nothing may be used in front of its arrival."""
+    say("cold caches", case)
+    E, N, Kd, _, _ = case
+    _, counts, _, xc, xs, wc, ws = make_product(*case)
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    x, x_scale, gl = dev(ref.pack(xc)), dev(xs), dev(counts.astype(np.int64))
+    acc = ref.products(ref.values(xc, xs), ref.values(wc, ws), counts)
+    other = torch.empty(1 << 28, dtype=torch.float32, device=DEV)
+    first = None
+    for i in range(12):
+        other.fill_(i)
+        got = both_products(K, E, N, Kd, x, x_scale, w, s, gl)
+        if first is None:
+            check_both(got, acc)
+            first = got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))

@@ -267,3 +267,40 @@ def test_launches_larger_than_there_are(lib):
     assert lib.moe355_format_cast_mx(P, P, 32768, 1 << 16, 64, P, P, None) == -2
     gmm = lambda rows, n: lib.moe355_gmm_mx(P, P, P, 4, P, P, P, 1, rows, 64, n, 2, P, 1, None, 0, None)
     assert gmm((1 << 31) - 1, 1 << 20) == -2
+
+
+def test_tiles_wait_for_the_tokens_of_their_first_window(tmp_path):
+    """The compiler orders loads to LDS only by what it sees, and the kernel's own wait counts loads: in front of the first barrier
+    the four loads of the first window's tokens must have landed, whatever order the others were put in."""
+    import subprocess
+
+    from test_abi_and_host import _code_objects
+    from vllm_ascend_amd import _lib
+
+    data, kernels = open(_lib.LIB_PATH, "rb").read(), 0
+    for at in _code_objects(data):
+        if b"gmm_mx_tiled_kernel" not in data[at:at + (1 << 22)]:
+            continue
+        part = tmp_path / "code"
+        part.write_bytes(data[at:at + (1 << 22)])
+        text = subprocess.run(["/opt/rocm/llvm/bin/llvm-objdump", "-d", "--mcpu=gfx950", str(part)], capture_output=True, text=True).stdout
+        for body in text.split("\n\n"):
+            lines = body.strip().split("\n")
+            if "gmm_mx_tiled_kernel" not in lines[0]:
+                continue
+            kernels += 1
+            pending, tokens = [], 0  # loads on their way, oldest first: True is one to LDS
+            for line in lines[1:]:
+                op = line.split("//")[0].split()
+                if not op:
+                    continue
+                if op[0].startswith(("buffer_load", "global_load", "scratch_", "buffer_store", "global_store")):
+                    pending.append(op[-1] == "lds")
+                    tokens += op[-1] == "lds"
+                elif op[0] == "s_waitcnt" and "vmcnt" in line:
+                    left = int(line.split("vmcnt(")[1].split(")")[0])
+                    pending = pending[max(len(pending) - left, 0):]
+                elif op[0] == "s_barrier" and tokens:
+                    assert tokens == 8 and sum(pending) <= 4, lines[0]  # two windows asked for, one of them still on its way
+                    break
+    assert kernels == 6

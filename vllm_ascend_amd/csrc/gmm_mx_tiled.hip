@@ -232,13 +232,19 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     Weights held[2];
     const int own = threadIdx.x, end = windows - 1;
     auto cut = [&](int w) { return w < end ? w : end; };
-    // prologue: windows 0 and 1 on their way
+    // Prologue: windows 0 and 1 on their way, in this order: what waits for the scales of window 1 waits for the tokens of window 0
+    // (the compiler does not know that the reads of LDS depend on them, and would move a load of tokens behind the scales).
     fetch_weights(0, held[0]);
     fetch_weights(1, held[1]);
+    __builtin_amdgcn_sched_barrier(0);
     fetch_tokens(0, 0);
-    scales[own] = fetch_scale(0).get();
+    __builtin_amdgcn_sched_barrier(0);
+    const MxRowScales scale_first = fetch_scale(0);
     MxRowScales scale_next = fetch_scale(cut(1));
+    __builtin_amdgcn_sched_barrier(0);
     fetch_tokens(cut(1), 1);
+    __builtin_amdgcn_sched_barrier(0);
+    scales[own] = scale_first.get();
     // Window w: its tokens and weights have been asked for two windows ago, a step's weights when the step that had their
     // registers was done.  Behind the barrier everybody has read window w - 1, whose place in the ring window w + 2 takes.
     int slot = 0;

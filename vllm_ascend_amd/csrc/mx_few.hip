@@ -1,10 +1,10 @@
 // The MXFP4 experts of a few tokens: what one token costs is not the weight stream but launches, 2 to 4 us each on the GPU and 3.6 on
 // the host.  There are two here, and nothing is sorted: every (token, slot) pair has workgroups of its own.
 //
-//   few_up_kernel    a workgroup has a pair and 32 gate channels with their 32 up channels.  It quantises the pair's token itself,
-//                    into LDS, while its first weights are on their way, and its wavefronts share K.
-//   few_down_kernel  a workgroup has 32 channels of a token and all its slots, a wavefront or more each, so that the token's rows
-//                    meet in LDS and leave as one: the combine, and the counts of the experts by one more row of workgroups.
+//   mx_up_few_kernel    a workgroup has a pair and 32 gate channels with their 32 up channels.  It quantises the pair's token itself,
+//                       into LDS, while its first weights are on their way, and its wavefronts share K.
+//   mx_down_few_kernel  a workgroup has 32 channels of a token and all its slots, a wavefront or more each, so that the token's rows
+//                       meet in LDS and leave as one: the combine, and the counts of the experts by one more row of workgroups.
 //
 // The 32 columns of a product all have the pair's row; lanes 0 and 32 hold what is wanted.  An expert that several tokens chose is
 // read for each of them, which is what ends the use (mx_few_takes).  One token through 8 of 128 experts of 2048 x 768 takes 12 us on
@@ -137,7 +137,7 @@ struct FewHidden {
 };
 
 template <int DT>
-__global__ __launch_bounds__(256) void few_up_kernel(MxArgs a, MxFew f)
+__global__ __launch_bounds__(256) void mx_up_few_kernel(MxArgs a, MxFew f)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
     const int lane = threadIdx.x & 63, half = lane >> 5, pair = blockIdx.y, tiles = (int)(a.N / 32);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void few_up_kernel(MxArgs a, MxFew f)
 }
 
 template <int DT>
-__global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(MxArgs a, MxFew f, int parts)
+__global__ __launch_bounds__(64 * kFewWaves) void mx_down_few_kernel(MxArgs a, MxFew f, int parts)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
     float* const sums = (float*)few_lds;  // [slots][parts][32]
@@ -268,11 +268,11 @@ int mx_few(const MxArgs& up, const MxArgs& down, const MxFew& f, int dtype, int6
     const dim3 down_grid((unsigned)(down.N / 32), (unsigned)tokens + 1);
     const size_t down_lds = (size_t)f.top_k * parts * 32 * 4;
     if (dtype == MOE355_DT_BF16) {
-        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_BF16>, up_grid, up_threads, lds, st, up, f);
-        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_BF16>, down_grid, down_threads, down_lds, st, down, f, parts);
+        hipLaunchKernelGGL(mx_up_few_kernel<MOE355_DT_BF16>, up_grid, up_threads, lds, st, up, f);
+        hipLaunchKernelGGL(mx_down_few_kernel<MOE355_DT_BF16>, down_grid, down_threads, down_lds, st, down, f, parts);
     } else {
-        hipLaunchKernelGGL(few_up_kernel<MOE355_DT_F16>, up_grid, up_threads, lds, st, up, f);
-        hipLaunchKernelGGL(few_down_kernel<MOE355_DT_F16>, down_grid, down_threads, down_lds, st, down, f, parts);
+        hipLaunchKernelGGL(mx_up_few_kernel<MOE355_DT_F16>, up_grid, up_threads, lds, st, up, f);
+        hipLaunchKernelGGL(mx_down_few_kernel<MOE355_DT_F16>, down_grid, down_threads, down_lds, st, down, f, parts);
     }
     return launch_status();
 }
