@@ -865,11 +865,22 @@ def _scale_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
     return _bytes(t, name, "float8_e8m0fnu")
 
 
-def _flat(t: torch.Tensor, name: str, alignment: int = 16) -> torch.Tensor:
-    """Contiguous, on the GPU, and starting where the kernels' wide loads may start (a view into another tensor need not)."""
-    if t.is_cuda and t.is_contiguous() and t.data_ptr() % alignment == 0:
+def _index(t: torch.Tensor, name: str) -> int:
+    """The GPU that a tensor is on."""
+    index = t.get_device()
+    if index < 0:
+        _dev(t, name)
+    return index
+
+
+def _flat(t: torch.Tensor, name: str, index: int, alignment: int = 16) -> torch.Tensor:
+    """Contiguous, on GPU `index`, and starting where the kernels' wide loads may start (a view into another tensor need not)."""
+    if t.get_device() != index:
+        _dev(t, name)
+        raise RuntimeError(f"operands on different devices: {name} {tuple(t.shape)} {t.dtype} is on {t.device}, the rows on GPU {index}")
+    if t.is_contiguous() and t.data_ptr() % alignment == 0:
         return t
-    t = _dev(t, name)
+    t = t.contiguous()
     return t if t.data_ptr() % alignment == 0 else t.clone()
 
 
@@ -885,13 +896,6 @@ def _call(index: int, name: str, *args) -> None:
         check(rc, name)
 
 
-def _on(index: int, *others) -> None:
-    for t in others:
-        if t is not None and t.get_device() != index:
-            raise RuntimeError(f"operands on different devices: the rows on device {index}, a {tuple(t.shape)} {t.dtype} tensor on "
-                               f"{t.device}")
-
-
 def _rows_of(x: torch.Tensor, op: str, multiple: int) -> tuple[int, int]:
     shape = x.shape
     if not shape or shape[-1] == 0 or shape[-1] % multiple:
@@ -903,11 +907,12 @@ def dynamic_mx_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 / fp16 / fp32 [..., K] -> (codes uint8 [..., K / 2], E8M0 scales uint8 [..., K / 32])."""
     dt = _dt(x, "x")
     rows, cols = _rows_of(x, "dynamic_mx_quant", MX_BLOCK)
-    x = _flat(x, "x")
+    index = _index(x, "x")
+    x = _flat(x, "x", index)
     lead = x.shape[:-1]
-    codes = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((*lead, cols // MX_BLOCK), dtype=torch.uint8, device=x.device)
-    _call(x.get_device(), "moe355_dynamic_mx_quant", x.data_ptr(), dt, rows, cols, codes.data_ptr(), scale.data_ptr())
+    codes = x.new_empty((*lead, cols // 2), dtype=torch.uint8)
+    scale = codes.new_empty((*lead, cols // MX_BLOCK))
+    _call(index, "moe355_dynamic_mx_quant", x.data_ptr(), dt, rows, cols, codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -920,10 +925,9 @@ def mx_dequant(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = to
     lead = codes.shape[:-1]
     if scale.shape != (*lead, half * 2 // MX_BLOCK):
         raise ValueError(f"mx_dequant: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
-    codes, scale = _flat(codes, "codes", 4), _dev(scale, "scale")
-    index = codes.get_device()
-    _on(index, scale)
-    out = torch.empty((*lead, half * 2), dtype=dtype, device=codes.device)
+    index = _index(codes, "codes")
+    codes, scale = _flat(codes, "codes", index, 4), _flat(scale, "scale", index, 1)
+    out = codes.new_empty((*lead, half * 2), dtype=dtype)
     _call(index, "moe355_mx_dequant", codes.data_ptr(), scale.data_ptr(), rows, half * 2, out.data_ptr(), _DT[dtype])
     return out
 
@@ -945,20 +949,19 @@ def add_rms_norm_quant(x1, x2, gamma, beta=None, epsilon=1e-6, kind=NORM_INT8):
         raise ValueError(f"{op}: beta {tuple(beta.shape)} {beta.dtype} does not match gamma {tuple(gamma.shape)} "
                          f"{gamma.dtype}")
     given = x1
-    x1 = _flat(x1, "x1")
-    x2 = None if x2 is None else _flat(x2, "x2")
-    gamma, beta = _flat(gamma, "gamma"), None if beta is None else _flat(beta, "beta")
-    index, dev = x1.get_device(), x1.device
-    _on(index, x2, gamma, beta)
+    index = _index(x1, "x1")
+    x1 = _flat(x1, "x1", index)
+    x2 = None if x2 is None else _flat(x2, "x2", index)
+    gamma, beta = _flat(gamma, "gamma", index), None if beta is None else _flat(beta, "beta", index)
     y = torch.empty_like(x1)
     x = torch.empty_like(x1) if x2 is not None else None
     q = scale = None
     if kind == NORM_INT8:
         q = torch.empty_like(x1, dtype=torch.int8)
-        scale = torch.empty(lead, dtype=torch.float32, device=dev)
+        scale = x1.new_empty(lead, dtype=torch.float32)
     elif kind == NORM_MXFP4:
-        q = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
-        scale = torch.empty((*lead, cols // MX_BLOCK), dtype=torch.uint8, device=dev)
+        q = x1.new_empty((*lead, cols // 2), dtype=torch.uint8)
+        scale = q.new_empty((*lead, cols // MX_BLOCK))
     dt = _DT[dtype]
     _call(index, "moe355_add_rms_norm_quant", x1.data_ptr(), _ptr(x2), gamma.data_ptr(), _ptr(beta), dt, DT_F32 if wide else dt,
           rows, cols, epsilon, kind, _ptr(x), y.data_ptr(), _ptr(q), _ptr(scale))
@@ -981,11 +984,11 @@ def format_cast_mx(codes: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tens
         raise ValueError(f"format_cast_mx: N must be a multiple of 32 and K of 64, got E = {E}, N = {n}, K = {k}")
     if scale.shape != (E, n, k // MX_BLOCK):
         raise ValueError(f"format_cast_mx: codes {tuple(codes.shape)} and scales {tuple(scale.shape)} do not belong together")
-    codes, scale = _flat(codes, "weight"), _dev(scale, "scale")
-    _on(codes.get_device(), scale)
+    index = _index(codes, "weight")
+    codes, scale = _flat(codes, "weight", index), _flat(scale, "scale", index, 1)
     out = torch.empty_like(codes)
-    out_scale = torch.empty((E, n, mx_scale_columns(k)), dtype=torch.uint8, device=codes.device)
-    _call(codes.get_device(), "moe355_format_cast_mx", codes.data_ptr(), scale.data_ptr(), E, n, k, out.data_ptr(),
+    out_scale = codes.new_empty((E, n, mx_scale_columns(k)))
+    _call(index, "moe355_format_cast_mx", codes.data_ptr(), scale.data_ptr(), E, n, k, out.data_ptr(),
           out_scale.data_ptr())
     return out, out_scale
 
@@ -996,7 +999,8 @@ def _mx_weights(op, weight, weight_scale, n_multiple):
     shape = weight.shape
     if len(shape) != 3:
         raise ValueError(f"{op}: weight must be [E, N, K / 2] (format_cast_mx), got {tuple(shape)}")
-    E, n, k = shape[0], shape[1], shape[2] * 2
+    E, n, half = shape
+    k = half * 2
     if not E or not n or not k or n % n_multiple or k % 64:
         raise ValueError(f"{op}: N must be a multiple of {n_multiple} and K of 64, got E = {E}, N = {n}, K = {k}")
     if weight_scale.shape != (E, n, mx_scale_columns(k)):
@@ -1034,13 +1038,13 @@ def _mx_product(op, entry, x, x_scale, weight, weight_scale, group_list, group_l
         rows = row_map.numel()
         if rows and not x_rows:
             raise ValueError(f"{op}: row_map names {rows} rows of an empty x")
-        row_map = _dev(row_map, "row_map")
-    x, x_scale = _flat(x, "x"), _dev(x_scale, "x_scale")
-    weight, weight_scale = _flat(weight, "weight"), _flat(weight_scale, "weight_scale")
+    index = _index(x, "x")
+    x, x_scale = _flat(x, "x", index), _flat(x_scale, "x_scale", index, 1)
+    weight, weight_scale = _flat(weight, "weight", index), _flat(weight_scale, "weight_scale", index)
+    if row_map is not None:
+        row_map = _flat(row_map, "row_map", index, 4)
     if group_list is not None:
-        group_list = _gl(group_list)
-    index = x.get_device()
-    _on(index, x_scale, weight, weight_scale, group_list, row_map)
+        group_list = _gl(_flat(group_list, "group_list", index, 4))
     list_type = _gl_type(group_list_type)
 
     def call(*outputs):
@@ -1049,25 +1053,24 @@ def _mx_product(op, entry, x, x_scale, weight, weight_scale, group_list, group_l
         _call(index, entry, x.data_ptr(), x_scale.data_ptr(), _ptr(row_map), x_rows, weight.data_ptr(), weight_scale.data_ptr(),
               _ptr(group_list), list_type, rows, k, n, E, *outputs, _ptr(ws), nbytes)
 
-    return n, call, rows, x.device
+    return n, call, rows, x
 
 
 def gmm_mx(x, x_scale, weight, weight_scale, group_list, group_list_type, out_dtype=torch.bfloat16, row_map=None):
     """MXFP4 rows [M, K / 2] times their experts' weights [E, N, K / 2] -> 16-bit [rows, N].  row_map: the row of x of every
     sorted row; without it the rows of x are sorted by expert.  group_list None: one expert, which has all rows."""
-    n, call, rows, device = _mx_product("gmm_mx", "moe355_gmm_mx", x, x_scale, weight, weight_scale, group_list, group_list_type,
-                                        row_map, 0)
-    out = torch.empty((rows, n), dtype=_half_dtype(out_dtype), device=device)
+    n, call, rows, like = _mx_product("gmm_mx", "moe355_gmm_mx", x, x_scale, weight, weight_scale, group_list, group_list_type,
+                                      row_map, 0)
+    out = like.new_empty((rows, n), dtype=_half_dtype(out_dtype))
     call(out.data_ptr(), _DT[out_dtype])
     return out
 
 
 def gmm_mx_swiglu_quant(x, x_scale, weight, weight_scale, group_list, group_list_type, swiglu_limit=0.0, row_map=None):
     """... with the gate_up weights [E, 2 I, K / 2], through SwiGLU to MXFP4: (codes [rows, I / 2], scales [rows, I / 32])."""
-    n, call, rows, device = _mx_product("gmm_mx_swiglu_quant", "moe355_gmm_mx_swiglu_quant", x, x_scale, weight, weight_scale,
-                                        group_list, group_list_type, row_map, 1)
-    out = torch.empty((rows, n // 4), dtype=torch.uint8, device=device)
-    out_scale = torch.empty((rows, n // 64), dtype=torch.uint8, device=device)
+    n, call, rows, like = _mx_product("gmm_mx_swiglu_quant", "moe355_gmm_mx_swiglu_quant", x, x_scale, weight, weight_scale,
+                                      group_list, group_list_type, row_map, 1)
+    out, out_scale = like.new_empty((rows, n // 4)), like.new_empty((rows, n // 64))
     call(swiglu_limit, out.data_ptr(), out_scale.data_ptr())
     return out, out_scale
 
@@ -1095,18 +1098,18 @@ def mx_experts(x, x_scale, topk_ids, topk_weights, w13, w13_scale, w2, w2_scale,
     if residual is not None:
         if residual.dtype != dtype or residual.shape != (T, H):
             raise ValueError(f"{op}: residual must be {dtype} of shape {(T, H)}, got {residual.dtype} {tuple(residual.shape)}")
-        residual = _flat(residual, "residual")
-    x, x_scale = _flat(x, "x"), None if x_scale is None else _dev(x_scale, "x_scale")
-    w13, w13_scale = _flat(w13, "w13"), _flat(w13_scale, "w13_scale")
-    w2, w2_scale, index = _flat(w2, "w2"), _flat(w2_scale, "w2_scale"), x.get_device()
-    topk_ids, topk_weights = _dev(topk_ids, "topk_ids"), _dev(topk_weights, "topk_weights")
-    _on(index, x_scale, topk_ids, topk_weights, w13, w13_scale, w2, w2_scale, residual)
-    k, dev = topk_ids.shape[1], x.device
-    out = torch.empty((T, H), dtype=dtype, device=dev)
-    tokens = (torch.empty if T else torch.zeros)((E,), dtype=torch.int64, device=dev)
+    index = _index(x, "x")
+    x, x_scale = _flat(x, "x", index), None if x_scale is None else _flat(x_scale, "x_scale", index, 1)
+    w13, w13_scale = _flat(w13, "w13", index), _flat(w13_scale, "w13_scale", index)
+    w2, w2_scale = _flat(w2, "w2", index), _flat(w2_scale, "w2_scale", index)
+    topk_ids, topk_weights = _flat(topk_ids, "topk_ids", index, 4), _flat(topk_weights, "topk_weights", index, 2)
+    residual = None if residual is None else _flat(residual, "residual", index)
+    k = topk_ids.shape[1]
+    out = topk_weights.new_empty((T, H))
+    tokens = (x.new_empty if T else x.new_zeros)((E,), dtype=torch.int64)
     if T:
         nbytes = _lib.load().moe355_mx_experts_workspace(T, k, H, I, E, int(x_scale is not None))
-        ws = _workspace(nbytes, dev)
+        ws = _workspace(nbytes, x.device)
         _call(index, "moe355_mx_experts", x.data_ptr(), _ptr(x_scale), _DT[dtype], T, H, topk_ids.data_ptr(),
               topk_weights.data_ptr(), k, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), I, E,
               swiglu_limit, _ptr(residual), tokens.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)

@@ -270,7 +270,7 @@ def _mx_quant_matmul(x1, x2, scale, offset, pertoken_scale, bias, output_dtype):
     if x2.dim() != 2 or scale.dim() != 2:
         raise ValueError("npu_quant_matmul: MXFP4 weights are [N, K / 2], their scales [N, columns] (npu_format_cast_mx)")
     lead = x1.shape[:-1]
-    rows = x1.reshape(-1, x1.shape[-1])
-    out = kernels.gmm_mx(rows, pertoken_scale.reshape(-1, pertoken_scale.shape[-1]), x2.unsqueeze(0), scale.unsqueeze(0),
-                         None, 0, output_dtype or torch.bfloat16)
-    return out.reshape(*lead, x2.shape[0])
+    if len(lead) != 1:
+        x1, pertoken_scale = x1.reshape(-1, x1.shape[-1]), pertoken_scale.reshape(-1, pertoken_scale.shape[-1])
+    out = kernels.gmm_mx(x1, pertoken_scale, x2.unsqueeze(0), scale.unsqueeze(0), None, 0, output_dtype or torch.bfloat16)
+    return out if len(lead) == 1 else out.reshape(*lead, x2.shape[0])
