@@ -252,8 +252,7 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
         const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
         scales[slot1 * (2 * kTileRows) + own] = scale_next.get();
         // behind this window's tokens: the next window's 4 loads of tokens and 10 of weights, at least
-        asm volatile("s_waitcnt vmcnt(14) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+        asm volatile("s_waitcnt vmcnt(14) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         scale_next = fetch_scale(cut(w + 2));
         __builtin_amdgcn_sched_barrier(0);
@@ -279,8 +278,7 @@ __global__ __launch_bounds__(kThreads, 2) void gmm_mx_tiled_kernel(MxArgs a, MxM
     __builtin_amdgcn_s_setprio(0);
     // The results go through LDS, which turns them into whole lines: once the loads past the end have landed and everybody has
     // read the last window.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const bool exists = row0 + t * 32 + row_in < row1;
