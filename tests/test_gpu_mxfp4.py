@@ -897,3 +897,17 @@ def test_products_on_cold_caches(K, case):
             check_both(got, acc)
             first = got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("E,rows", [(3, 9), (3, 900), (600, 4000), (300, 40)])
+def test_counts_far_past_the_last_row_behind_other_groups(K, E, rows):
+    """A count that no sum of 64 bits holds is cut like any other, in every form: the rest of the rows are its expert's."""
+    say("far counts", E, rows)
+    N, Kd, first = 1600 if E == 3 else 64, 64, 5
+    _, _, _, xc, xs, wc, ws = make_product(E, N, Kd, rows, "even")
+    w, s = K.format_cast_mx(dev(ref.pack(wc)), dev(ws))
+    most = (1 << 63) - 1
+    acc = ref.products(ref.values(xc, xs), ref.values(wc, ws), [first, rows - first] + [0] * (E - 2))
+    for count, behind in ((most, 0), (most, most), (most - first, 1), (most - first + 1, 0), (most - rows, most)):
+        gl = torch.tensor([first, count] + [behind] * (E - 2), device=DEV)
+        check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, gl), acc)

@@ -109,7 +109,7 @@ __device__ __forceinline__ void mx_expert_rows(const MxArgs& a, int e, int lane,
         for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
         row0 = total;
         const int64_t n = a.group_list[e];
-        row1 = row0 + (n > 0 ? n : 0);
+        row1 = row0 + (n < 0 ? 0 : n < a.rows ? n : a.rows);
     }
     row0 = row0 < 0 ? 0 : row0 > a.rows ? a.rows : row0;
     row1 = row1 < row0 ? row0 : row1 > a.rows ? a.rows : row1;
