@@ -911,3 +911,16 @@ def test_counts_far_past_the_last_row_behind_other_groups(K, E, rows):
     for count, behind in ((most, 0), (most, most), (most - first, 1), (most - first + 1, 0), (most - rows, most)):
         gl = torch.tensor([first, count] + [behind] * (E - 2), device=DEV)
         check_both(both_products(K, E, N, Kd, dev(ref.pack(xc)), dev(xs), w, s, gl), acc)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+def test_layer_of_codes_under_the_names_of_their_types(ops, dtype):
+    say("layer of named codes", dtype)
+    layer, _, _ = build(8, 2, 512, 256, dtype)
+    g = torch.Generator().manual_seed(7)
+    x, logits = torch.randn(30, 512, generator=g).to(dtype).to(DEV), torch.randn(30, 8, generator=g).to(DEV)
+    want = layer(x, logits)
+    codes, scale = ops.npu_dynamic_mx_quant(x)
+    layer.ascend_pertoken_scale = scale.view(torch.float8_e8m0fnu)
+    for given in (codes, codes.view(torch.float4_e2m1fn_x2)):
+        assert torch.equal(layer(given, logits), want)

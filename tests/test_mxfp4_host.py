@@ -304,3 +304,28 @@ def test_tiles_wait_for_the_tokens_of_their_first_window(tmp_path):
                     assert tokens == 8 and sum(pending) <= 4, lines[0]  # two windows asked for, one of them still on its way
                     break
     assert kernels == 6
+
+
+@pytest.mark.parametrize("name", [torch.uint8, FP4], ids=str)
+def test_layer_asks_the_router_for_weights_of_the_model_type(name):
+    """Rows that the caller has quantised, under either of the names of their type."""
+    from vllm_ascend_amd.fused_moe.contracts import FusedExpertsResult, FusedMoEConfig
+    from vllm_ascend_amd.fused_moe.layer import AscendRoutedExperts
+    from vllm_ascend_amd.fused_moe.router import AscendFusedTopKRouter
+    from vllm_ascend_amd.quantization import get_scheme_class
+
+    asked = []
+
+    class Router(AscendFusedTopKRouter):
+        def select_experts(self, hidden_states, router_logits, **kw):
+            asked.append(kw["weights_dtype"])
+            return torch.ones(3, 1), torch.zeros(3, 1, dtype=torch.int32)
+
+    for dtype in (torch.bfloat16, torch.float16):
+        scheme = get_scheme_class("W4A4_MXFP4", "moe")(in_dtype=dtype)
+        scheme.apply = lambda layer, x, *a: FusedExpertsResult(routed_out=x)
+        layer = AscendRoutedExperts(FusedMoEConfig(num_experts=2, experts_per_token=1, hidden_dim=64, intermediate_size_per_partition=64),
+                                    scheme, Router(1, 2), device="cpu")
+        layer.ascend_pertoken_scale = torch.zeros(3, 2, dtype=torch.uint8)
+        layer(torch.zeros(3, 32, dtype=torch.uint8).view(name), torch.zeros(3, 2))
+        assert asked.pop() is dtype and not asked

@@ -14,6 +14,9 @@ from .layer_call import layer_call
 from .moe_comm_method import setup_moe_comm_method
 from .router import AscendFusedTopKRouter
 
+# types of hidden states that the caller has quantised
+_QUANTISED = (torch.int8, torch.uint8, getattr(torch, "float4_e2m1fn_x2", torch.uint8))
+
 
 class AscendRoutedExperts(torch.nn.Module):
     def __init__(self, moe_config: FusedMoEConfig, quant_method: AscendMoEScheme, router: AscendFusedTopKRouter,
@@ -123,10 +126,10 @@ class AscendRoutedExperts(torch.nn.Module):
         if self.use_fused_small_batch and fused is not None and fused(self, hidden_states, router_logits, self.router):
             return self.quant_method.apply_small_batch(self, hidden_states, router_logits, self.router,
                                                        self.shared_experts, None)
-        # int8 hidden states (uint8: MXFP4 codes) = activations the caller quantised (their scales in
-        # ascend_pertoken_scale): the routing weights then take the model dtype of the scheme
+        # int8 hidden states (uint8 or float4_e2m1fn_x2: MXFP4 codes) = activations the caller quantised (their scales
+        # in ascend_pertoken_scale): the routing weights then take the model dtype of the scheme
         weights_dtype = None
-        if hidden_states.dtype in (torch.int8, torch.uint8):
+        if hidden_states.dtype in _QUANTISED:
             weights_dtype = getattr(self.quant_method, "in_dtype", torch.bfloat16)
         topk_weights, topk_ids = self.router.select_experts(
             hidden_states, router_logits, enable_force_load_balance=self.enable_force_load_balance,
