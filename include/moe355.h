@@ -631,7 +631,8 @@ int moe355_gmm_mx_swiglu_quant(const uint8_t *x, const uint8_t *x_scale, const i
  * moe355_gmm_mx and moe355_token_unpermute in one call, the same bits where fp32 holds the products' sums exactly (blocks of a row
  * some powers of two apart; otherwise the order of a sum depends on the form that the sizes choose).  topk_ids [T, k], topk_weights [T, k] of dtype; residual
  * [T, hidden] of dtype or NULL; expert_tokens [E] receives the counts; out [T, hidden] of dtype (bf16 / fp16).  hidden and
- * intermediate are multiples of 64, E at most 2048, k at most 64. */
+ * intermediate are multiples of 64, hidden at most 2^20, intermediate 2^19, E 2048, k 64; T below 2^24, T * hidden / 2 and T * k *
+ * intermediate / 2 below 4 GiB less 1 MiB, (T * k / 128 + E) * hidden / 256 below 2^24. */
 size_t moe355_mx_experts_workspace(int64_t num_tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts,
                                    int quantised);
 int moe355_mx_experts(const void *x, const uint8_t *x_scale, int dtype, int64_t num_tokens, int64_t hidden,

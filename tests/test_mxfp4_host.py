@@ -329,3 +329,12 @@ def test_layer_asks_the_router_for_weights_of_the_model_type(name):
         layer.ascend_pertoken_scale = torch.zeros(3, 2, dtype=torch.uint8)
         layer(torch.zeros(3, 32, dtype=torch.uint8).view(name), torch.zeros(3, 2))
         assert asked.pop() is dtype and not asked
+
+
+@pytest.mark.parametrize("T,H,k,E,fits", [(8190, 1 << 20, 64, 8, False), (8190, 1 << 20, 63, 8, True), (1 << 24, 64, 1, 8, False),
+                                          ((1 << 24) - 1, 64, 1, 8, True)])
+def test_experts_of_more_threads_than_a_launch_has(lib, T, H, k, E, fits):
+    """The down product's tiles, or the combine's tokens: refused before the first launch, and no workspace asked for."""
+    assert (lib.moe355_mx_experts_workspace(T, k, H, 64, E, 0) > 0) == fits
+    if not fits:
+        assert lib.moe355_mx_experts(P, None, 1, T, H, P, P, k, P, P, P, P, 64, E, 0.0, None, P, P, P, 1 << 60, None) == -2

@@ -275,6 +275,13 @@ MxMap mx_map_in(void* workspace, int64_t rows, int num_experts);  // 256-byte al
 // the group list or in a list that a launch in front makes (mx_build_map, or the routing launch).
 enum MxForm { MX_STREAM, MX_TILES, MX_LISTED };
 MxForm mx_form(int64_t rows, int64_t n, int num_experts, bool swiglu, bool grouped);
+// a launch has at most 2^32 - 1 threads: 256 for every tile that the product may have
+constexpr int64_t kMxMostGroups = 0xffffffff / 256;
+inline bool mx_launches(int64_t rows, int64_t n, int num_experts, bool swiglu)
+{
+    const int64_t columns = swiglu ? (n / 64 + 3) / 4 : (n / 32 + 7) / 8;
+    return columns * (mx_most_tiles(rows, num_experts) + 8) <= kMxMostGroups;
+}
 void mx_build_map(const MxArgs& a, const MxMap& map, hipStream_t st);
 int mx_check(const MxArgs& a, bool swiglu);
 // map: of MX_LISTED.  The arguments have been checked.

@@ -89,9 +89,7 @@ int mx_check(const MxArgs& a, bool swiglu)
         return MOE355_E_SHAPE;
     // rows of x are reached by offsets of 32 bits
     if (a.rows > 0x7fffffff || a.x_rows > 0x7fffffff || a.x_rows * (a.K / 2) > kMxNowhere) return MOE355_E_SHAPE;
-    // a launch has at most 2^32 - 1 threads
-    const int64_t columns = swiglu ? (a.N / 64 + 3) / 4 : (a.N / 32 + 7) / 8;
-    if (columns * (mx_most_tiles(a.rows, a.E) + 8) > 0xffffffff / 256) return MOE355_E_SHAPE;
+    if (!mx_launches(a.rows, a.N, a.E, swiglu)) return MOE355_E_SHAPE;
     if (a.rows == 0) return MOE355_OK;
     if (a.x_rows == 0 || !a.x || !a.x_scale || !a.w || !a.w_scale || (!a.group_list && a.E > 1) || !a.out || (swiglu && !a.out_scale))
         return MOE355_E_ARG;

@@ -48,8 +48,11 @@ bool bad_sizes(int64_t T, int k, int64_t H, int64_t I, int E)
 }
 bool unsupported(int64_t T, int k, int64_t H, int64_t I, int E)
 {
-    return H % 64 || I % 64 || H > (int64_t)1 << 20 || I > (int64_t)1 << 19 || k > 64 || E > 2048 || T > 0x7ffffffe / k ||
-           T * (H / 2) > kMxNowhere || T * k * (I / 2) > kMxNowhere;
+    if (H % 64 || I % 64 || H > (int64_t)1 << 20 || I > (int64_t)1 << 19 || k > 64 || E > 2048 || T > 0x7ffffffe / k ||
+        T * (H / 2) > kMxNowhere || T * k * (I / 2) > kMxNowhere)
+        return true;
+    // (the combine has a workgroup a token)
+    return T > kMxMostGroups || !mx_launches(T * k, 2 * I, E, true) || !mx_launches(T * k, H, E, false);
 }
 
 }  // namespace
