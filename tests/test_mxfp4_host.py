@@ -338,3 +338,36 @@ def test_experts_of_more_threads_than_a_launch_has(lib, T, H, k, E, fits):
     assert (lib.moe355_mx_experts_workspace(T, k, H, 64, E, 0) > 0) == fits
     if not fits:
         assert lib.moe355_mx_experts(P, None, 1, T, H, P, P, k, P, P, P, P, 64, E, 0.0, None, P, P, P, 1 << 60, None) == -2
+
+
+def test_device_operator_takes_mx_calls_for_what_they_say():
+    """An MX call of int8 rows or weights is not the int8 product; a type other than four bits is refused wherever it is named."""
+    from vllm_ascend_amd.device_op import DeviceOperator as D
+
+    E, N, K, M = 2, 64, 128, 5
+    x, xs = torch.zeros(M, K // 2, dtype=torch.uint8), torch.zeros(M, K // 32, dtype=torch.uint8)
+    w, ws = torch.zeros(E, N, K // 2, dtype=torch.uint8), torch.zeros(E, N, 8, dtype=torch.uint8)
+    gl = torch.tensor([2, 3])
+    int8 = dict(x=torch.zeros(M, K, dtype=torch.int8), xs=torch.ones(M), w=torch.zeros(E, K, N, dtype=torch.int8), ws=torch.ones(E, N))
+
+    def down(x=x, xs=xs, w=w, ws=ws, **kw):
+        return D.npu_grouped_matmul_gmm2(hidden_states=x, weight=[w], weight_scale=[ws], per_token_scale=xs, group_list=gl,
+                                         group_list_type=1, input_dtype=torch.bfloat16, use_mxfp_quant=True, **kw)
+
+    def up(x=x, xs=xs, w=w, ws=ws, **kw):
+        return D.npu_grouped_matmul_swiglu_quant(x=x, weight=w, group_list=gl, weight_scale=ws, x_scale=xs, group_list_type=1,
+                                                 use_mxfp_quant=True, **kw)
+
+    for call in (up, down):
+        for name in (None, FP4, torch.uint8):
+            with pytest.raises(RuntimeError, match="GPU"):
+                call(act_quant_type=name, weight_quant_type=name, mxfp_quant_dtype=name)
+        for name in ("act_quant_type", "weight_quant_type", "mxfp_quant_dtype"):
+            with pytest.raises(NotImplementedError):
+                call(**{name: torch.float8_e4m3fn})
+        with pytest.raises(TypeError):
+            call(**int8)
+        with pytest.raises(TypeError):
+            call(x=int8["x"], xs=int8["xs"])
+        with pytest.raises(TypeError):
+            call(w=int8["w"], ws=int8["ws"])

@@ -68,6 +68,8 @@ class MI355XDeviceAdaptor:
         """``group_list_type`` (not in the reference, whose op only takes a running sum): 1 hands the
         per-expert counts of the dispatcher to the kernel as they are, which saves the cumsum launch."""
         if use_mxfp_quant:
+            _fp4(weight_quant_type)
+            _fp4(mxfp_quant_dtype)
             out, out_scale = npu_ops.npu_grouped_matmul_swiglu_quant_v2(
                 x, weight, weight_scale, x_scale, group_list, bias=bias, quant_dtype=_fp4(act_quant_type),
                 group_list_type=group_list_type, swiglu_limit=swiglu_limit)
@@ -103,6 +105,11 @@ class MI355XDeviceAdaptor:
                                 mxfp_quant_dtype=None):
         if use_mxfp_quant:
             _fp4(act_quant_type)
+            _fp4(weight_quant_type)
+            _fp4(mxfp_quant_dtype)
+            if not npu_ops._is_mx(hidden_states):
+                raise TypeError(f"MXFP MoE quantization on MI355X: uint8 or float4_e2m1fn_x2 codes expected but got "
+                                f"{hidden_states.dtype}")
             fallback_output_dtype = input_dtype if input_dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
         if fallback_output_dtype is None:
             first = weight_scale[0] if isinstance(weight_scale, list) else weight_scale
