@@ -100,17 +100,21 @@ int mx_check(const MxArgs& a, bool swiglu)
 MxForm mx_form(int64_t rows, int64_t n, int num_experts, bool swiglu, bool grouped)
 {
     // Streaming has no list to make and splits K, so it is for calls that tiles would not fill the chip with: up to 512 workgroups
-    // of 32 rows x 64 channels, and for fewer than 4 rows an expert.  us streamed / tiles: 8 experts of 1024 -> 2 x 1408, 64 / 128 /
-    // 256 tokens of 2 slots 7.6 / 10.9 / 18.3 against 7.8 / 10.5 / 13.1 (352, 352, 704 workgroups), of 1408 -> 1024 5.1 / - / 6.1
-    // against 6.3 / - / 9.9; one expert of 7168 -> 4096, 128 / 256 / 512 / 1024 rows 10.7 / 19.2 / 30.0 / 57.2 against 26.6 /
-    // 32.3 / 33.7 / 36.5.  128 experts of 2048 -> 2 x 768, 4 / 16 / 64 / 256 tokens of 8 slots 10.5 / 26.1 / 34.6 / 39.5 against
-    // 14.8 / 27.7 / 34.7 / 39.0; skewed (Zipf(1.1)) 64 / 256 tokens 25.0 / 64.4 against 27.2 / 41.3, 256 experts of 7168 -> 2 x
-    // 2048 128 / 512 tokens 249 / 690 against 189 / 317: a hot expert's many rows go through its few workgroups.
+    // of 32 rows x 64 channels, and for fewer than 4 rows an expert.  us streamed / tiles, on the same buffers again: 8 experts of 1024
+    // -> 2 x 1408, 64 / 128 / 256 tokens of 2 slots 6.5 / 7.7 / 9.8 against 8.1 / 10.9 / 12.9 (352, 352, 704 workgroups), of 1408 ->
+    // 1024 64 / 256 tokens 5.2 / 5.3 against 7.0 / 9.8; one expert of 7168 -> 4096, 128 / 256 / 512 / 1024 rows 9.8 / 16.6 / 30.4 / 56
+    // against 23.8 / 26.4 / 27.2 / 28.1 (256 to 2048 workgroups; between 512 and 1024 either may be ahead).  128 experts of 2048 -> 2 x
+    // 768, 4 / 16 / 64 / 256 tokens of 8 slots 10.3 / 27.9 / 36.0 / 41.1 against 16.3 / 28.8 / 37.5 / 39.7.  Skewed (Zipf(1.1)) the same
+    // with 64 / 256 tokens 25.9 / 65.8 against 28.8 / 39.9, 256 experts of 7168 -> 2 x 2048 with 64 / 127 / 128 tokens 157 / 223 / 218
+    // against 171 / 217 / 193 and of 2048 -> 7168 with 64 / 127 77 / 111 against 86 / 108: a hot expert's many rows go through its few
+    // workgroups, which pays for tiles from 4 rows an expert on.  (The call that this rule serves worst has one slot a token and all
+    // tokens at one expert: 1000 of them at one of 256, 274 against 55.  Workgroups for more chunks of every expert's rows are no
+    // remedy: six instead of one, 64 tokens of 256 experts 523 -> 630 uniform, 157 -> 193 skewed.)
     const int64_t pairs = swiglu ? n / 64 : (n / 32 + 1) / 2, chunks = (rows + 32 * (int64_t)num_experts - 1) / (32 * (int64_t)num_experts);
     if (rows < 4 * (int64_t)num_experts || pairs * num_experts * chunks <= 512) return MX_STREAM;
     // Finding the tiles in the product costs a workgroup for every tile that an expert might have, most of which end at once; a
-    // list takes a launch of 5 us in front.  Found / listed, us, at 3 / 6 / 12 / 25 / 33 thousand of them: 34.7 / 35.8 / 39.0
-    // / 50.6 / 38.3 against 38.6 / 39.1 / 41.6 / 54.4 / 32.5, the last two skewed 45.3 / 37.0 against 44.5 / 27.7.
+    // list takes a launch of 5 us in front.  Found / listed, us, at 3 / 6 / 12 / 25 / 33 thousand of them: 35.8 / 37.3 / 39.4
+    // / 52.0 / 38.0 against 38.3 / 40.7 / 43.3 / 53.0 / 33.2, the last two skewed 45.8 / 35.4 against 42.0 / 27.0.
     const int64_t columns = swiglu ? (n / 64 + 3) / 4 : (n / 32 + 7) / 8, tiles = (rows + kMxTileRows - 1) / kMxTileRows;
     return grouped && columns * num_experts * tiles > 16384 ? MX_LISTED : MX_TILES;
 }

@@ -5,12 +5,15 @@
 // accumulators a lane.  Tokens come through LDS, three windows of 256 K in a ring, by LDS-direct loads two windows ahead;
 // weights go straight from the caches to registers in the order of their storage, as far ahead (a step's when the step that had
 // its registers is done), since no other wavefront of the workgroup reads them.  A step of 64 K takes 8 matrix instructions of 32 cycles, 2 KiB of weights and 4 KiB of
-// tokens a wavefront: 64 of the 128 bytes a cycle that LDS gives, 48 of the 64 of the L1.  Two workgroups share a compute unit, so
-// that the vector instructions of one's epilogue run beside the other's matrix instructions.
+// tokens a wavefront: while the matrix units do not pause, 64 of the 128 bytes a cycle that LDS gives and 48 of the 64 that a compute
+// unit's L1 gets.  Two workgroups share a compute unit, so that the vector instructions of one's epilogue run beside the other's
+// matrix instructions.
 //
-// 65536 rows of 2048 -> 2 x 768 with SwiGLU 145 us (2.8 PFLOP/s), of 768 -> 2048 104 us (2.0; 3.7 TB/s), 2048 x 7168 x 4096 33 us (3.6),
-// 8192^3 258 us (4.3).  With the loads alone the first takes 107 us, with the products and the start of a tile alone 104, with the
-// epilogue 127: what is left is that neither hides all of the other.
+// us on the same buffers again / on buffers in turn: 65536 rows of 2048 -> 2 x 768 with SwiGLU 146 / 157 (2.8 / 2.6 PFLOP/s), of 768 ->
+// 2048 105 / 123 (2.0 / 1.7; 3.8 / 3.3 TB/s), both with the list's 5; 2048 x 7168 x 4096 35 / 40 (3.4 / 3.0), 8192^3 258 on the same
+// (4.3).  With the loads alone the first kernel takes 107, with the products and the start of a tile alone 104, with the epilogue 127:
+// what is left is that neither hides all of the other.  By the counters its matrix units are busy for 35 % of the cycles, its L1s get
+// 25 bytes a cycle, LDS loses 3 % to conflicts.
 #include "gmm_mx_stream.h"
 
 namespace moe355 {

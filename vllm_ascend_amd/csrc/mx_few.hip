@@ -7,8 +7,8 @@
 //                       meet in LDS and leave as one: the combine, and the counts of the experts by one more row of workgroups.
 //
 // The 32 columns of a product all have the pair's row; lanes 0 and 32 hold what is wanted.  An expert that several tokens chose is
-// read for each of them, which is what ends the use (mx_few_takes).  One token through 8 of 128 experts of 2048 x 768 takes 12 us on
-// the GPU (20 MB: 4 us; the two launches by themselves, behind an idle GPU, 6.8 and 5.8).
+// read for each of them, which is what ends the use (mx_few_takes).  One token through 8 of 128 experts of 2048 x 768 takes 16.6 us on
+// the GPU, 11.4 with the weights of the call before (20 MB: 4 us; the two launches by themselves 9.6 and 6.5, or 7.0 and 5.9).
 #include "mx_few.h"
 
 namespace moe355 {
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_down_few_kernel(MxArgs a, M
 bool mx_few_takes(int64_t tokens, int top_k, int64_t hidden, int64_t intermediate, int num_experts)
 {
     // A wavefront for every slot of a token, a row of x in LDS; and the launches that it saves are worth some 125 million weights of
-    // each projection in all, 50 million of them read again because several pairs have the same expert.  us on the GPU, here /
+    // each projection in all, 50 million of them read again because several pairs have the same expert.  us on the GPU (same buffers), here /
     // sorted (the host gains 6 of 23 in all of them), and those two numbers: 128 experts of 2048 x 768, 1 / 4 / 8 / 16 tokens of 8
     // slots 12 / 20.7 / 29.8 / 48.2 against 17 / 25 / 34.5 / 46.3 (13, 50, 100, 201; 0); 8 of 1024 x 1408, 1 / 8 / 16 / 32 tokens of 2
     // slots 9.5 / 10.5 / 13.5 / 21.2 against 16 / 17.8 / 18 / 18.2 (3, 23, 46, 92; 0, 12, 35, 81); 64 of 2048 x 1408, 4 / 8 tokens of 6

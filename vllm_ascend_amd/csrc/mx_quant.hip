@@ -9,7 +9,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int64_t kMostThreads = 0xffffffff;  // of a launch
 
-// HBM bound: 2 (4) bytes in and 17/32 out a value; 8192 rows of 7168 in 23 us, 6.5 TB/s.
+// HBM bound: 2 (4) bytes in and 17/32 out a value; 65536 rows of 7168 in 198 us, 6.0 TB/s.  (8192 rows, 149 MB, in 28 us; 23 on the same
+// buffers again, which the 256 MiB of the last cache hold.)
 template <int DT>
 __global__ __launch_bounds__(kThreads) void mx_quant_kernel(const char* __restrict__ x, int64_t pieces,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scale)
@@ -51,8 +52,9 @@ __global__ __launch_bounds__(kThreads) void mx_dequant_kernel(const uint32_t* __
 //
 // Squares, their sum and the norm itself are in 64 bits: a square of a 16-bit value is exact there, so the sum does not depend
 // on how the row is spread over lanes to any bit that reaches y, and y is what the formula gives, rounded to 32 and to 16 bits.
-// The launch is HBM bound all the same, 9 bytes a value to int8: 4096 rows of 7168 in 48 us, 5.5 TB/s (to MXFP4 40.6 us, 6.2 TB/s, where a
-// large copy reaches 5.0); a row of 7168 alone 5.1 us.
+// The launch is HBM bound all the same, 9 bytes a value to int8: 65536 rows of 7168 in 840 us, 5.0 TB/s (to MXFP4 690 us, 5.8 TB/s; a
+// large copy reaches 5.0).  4096 rows, 264 MB, take 59 us (50); 49 (41) on the same buffers again, part of which the last cache
+// holds.  A row of 7168 alone 5 us.
 //
 // y is rounded to 16 bits before it is quantised because that is what the next operators of the model see: the router's gate
 // and a shared expert read y, and quantising y later gives the same codes.
@@ -136,7 +138,8 @@ __global__ __launch_bounds__(1024) void norm_quant_kernel(NormArgs a)
         g.fetch(a.gamma, i);
         if (a.beta) b.fetch(a.beta, i);
     };
-    // non-temporal: 4096 rows of 7168 to int8 60 -> 55 us, to MXFP4 50 -> 43, 777 of 2048 5.3 -> 5.1 (of q as well: no difference)
+    // non-temporal: 4096 rows of 7168 to int8 60 -> 55 us, to MXFP4 50 -> 43, 777 of 2048 5.3 -> 5.1, on the same buffers again (of
+    // q as well: no difference)
     auto put = [&](v8u16* to, v8u16 v) { __builtin_nontemporal_store(v, to); };
     double sum = 0.0;
     if constexpr (NV > 0) {
@@ -258,7 +261,7 @@ NormShape norm_shape(int64_t cols)
     const int64_t nv = cols >> 3;
     const unsigned waves = (unsigned)((nv + 63) / 64);
     // Two pieces a thread from 512 on: 4096 rows of 7168 to int8 74.1 -> 65.9 us, to MXFP4 59.6 -> 56.6 (four 65.7, 56.5, but a row
-    // alone 7.7 instead of 6.3); 8192 rows of 2048 33.4 with one, 35.8 with two.
+    // alone 7.7 instead of 6.3); 8192 rows of 2048 33.4 with one, 35.8 with two (the same buffers again).
     if (nv <= 512) return {1, 64 * waves};
     if (nv <= 2048) return {2, 64 * ((waves + 1) / 2)};
     return {0, 1024};
